@@ -553,6 +553,84 @@ int mdx_heatmaps_to_keypoints(const float *maps, const float *boxes, const int *
                               int K, int M, float *out, mdx_stream_t stream);
 
 /* ---------------------------------------------------------------------
+ * Layers of the heads beyond the shipped model's convolutions, for serving
+ * and training (Detectron2 builds its box heads from torch.nn.Linear and its
+ * "LN" norms from layer norm; the reference's own configuration keeps to
+ * FastRCNNConvFCHead, M/model/config.py:21-94).  dtype codes: 0 = float32,
+ * 1 = float16, 3 = bfloat16; products accumulate in float32, outputs are
+ * rounded once.  bias, gamma, beta and their gradients are float32.  Matrices
+ * are row-major; ld* is the distance between rows in elements, at least the
+ * row's length, with any alignment.  An output must not overlap an input,
+ * except where it is exactly that buffer and the call says so.  No entry
+ * allocates or synchronises: all can be captured into a graph, and calls on
+ * several streams run side by side on workspaces of their own.
+ * ------------------------------------------------------------------- */
+enum {
+    MDX_ACT_NONE = 0,
+    MDX_ACT_RELU = 1,
+    MDX_ACT_GELU = 2,       /* z (1 + erf(z / sqrt 2)) / 2 */
+    MDX_ACT_GELU_TANH = 3,  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+    MDX_ACT_SILU = 4        /* z / (1 + exp(-z)) */
+};
+
+/* z = x w^T + bias + residual; out = act(z); pre (or NULL) = z.
+ * x (M,K), w (N,K), bias [N] or NULL, residual (M,N) or NULL, out / pre (M,N).
+ * out may be the residual's own buffer (same ldo).  workspace: where few
+ * output tiles would leave CUs idle, the reduction is split and joined through
+ * mdx_linear_workspace_bytes bytes (0 = not split); with less it is not
+ * split. */
+int64_t mdx_linear_workspace_bytes(int64_t M, int N, int K, int dtype);
+int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *bias, const void *residual,
+               int64_t ldr, int64_t M, int N, int K, int act, int dtype, void *pre, int64_t ldp, void *out, int64_t ldo,
+               void *workspace, int64_t workspace_bytes, mdx_stream_t stream);
+/* Its gradients, each computed where its pointer is not NULL: dz = grad act'(pre),
+ * rounded to dtype; dx = dz w, dw = dz^T x, dres = dz, dbias = the column sums
+ * of dz before that rounding.  pre may be NULL for MDX_ACT_NONE.  dres may be
+ * grad's own buffer (same lddr).  workspace: at least
+ * mdx_linear_backward_workspace_bytes (which gradients are needed as flags).
+ * Sums are taken in a fixed order: a call repeats bit for bit. */
+int64_t mdx_linear_backward_workspace_bytes(int64_t M, int N, int K, int act, int dtype, int need_x, int need_w,
+                                            int need_bias, int need_residual);
+int mdx_linear_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const void *w, int64_t ldw,
+                        const void *pre, int64_t ldp, int64_t M, int N, int K, int act, int dtype, void *dx,
+                        int64_t lddx, void *dw, int64_t lddw, float *dbias, void *dres, int64_t lddr, void *workspace,
+                        int64_t workspace_bytes, mdx_stream_t stream);
+
+/* The same layer with E weights over ragged groups of rows: rows of x (T,K)
+ * lie group by group, counts [E] (int32, on the device, never read by the
+ * host) of them each; w (E,N,K) and bias [E][N] are contiguous.  A negative
+ * count is taken as 0, and counts are cut where their sum passes T.  The rows
+ * behind the last group are left as they were in out / pre (zero_tail 0) or
+ * written as zeros (1).  E <= 4096. */
+int mdx_grouped_linear(const void *x, int64_t ldx, const void *w, const float *bias, const void *residual, int64_t ldr,
+                       const int *counts, int E, int64_t T, int N, int K, int act, int dtype, void *pre, int64_t ldp,
+                       void *out, int64_t ldo, int zero_tail, mdx_stream_t stream);
+/* dw (E,N,K) and dbias [E][N] of a group without rows are zeros; zero_tail
+ * holds for dx and dres. */
+int64_t mdx_grouped_linear_backward_workspace_bytes(int E, int64_t T, int N, int K, int act, int dtype, int need_x,
+                                                    int need_w, int need_bias, int need_residual);
+int mdx_grouped_linear_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const void *w,
+                                const void *pre, int64_t ldp, const int *counts, int E, int64_t T, int N, int K,
+                                int act, int dtype, void *dx, int64_t lddx, void *dw, float *dbias, void *dres,
+                                int64_t lddr, int zero_tail, void *workspace, int64_t workspace_bytes,
+                                mdx_stream_t stream);
+
+/* Layer norm of rows of D: out = (x - mean) rstd gamma + beta, biased
+ * variance, rstd = 1 / sqrt(var + eps).  gamma / beta [D] or NULL (1 / 0).
+ * mean / rstd [rows] or NULL: written for the backward pass.  out may be x's
+ * own buffer (same ldo). */
+int mdx_layer_norm(const void *x, int64_t ldx, const float *gamma, const float *beta, int64_t rows, int D, float eps,
+                   int dtype, void *out, int64_t ldo, float *mean, float *rstd, mdx_stream_t stream);
+/* dx (or NULL), dgamma = sum over rows of grad (x - mean) rstd (or NULL),
+ * dbeta = sum of grad (or NULL).  dx may be grad's own buffer (same lddx).
+ * workspace (for dgamma / dbeta): mdx_layer_norm_backward_workspace_bytes. */
+int64_t mdx_layer_norm_backward_workspace_bytes(int64_t rows, int D, int dtype);
+int mdx_layer_norm_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const float *mean,
+                            const float *rstd, const float *gamma, int64_t rows, int D, int dtype, void *dx,
+                            int64_t lddx, float *dgamma, float *dbeta, void *workspace, int64_t workspace_bytes,
+                            mdx_stream_t stream);
+
+/* ---------------------------------------------------------------------
  * Model handle: the whole Mask/Keypoint R-CNN forward as one C call.
  * Replaces Predictor.from_config (M/model/predict.py:31-44: build_model +
  * DetectionCheckpointer.load) and Predictor.__call__'s model(inputs)

@@ -106,6 +106,18 @@ SIGNATURES = {
     "mdx_model_debug_arena": (I32, [P, P, ctypes.c_char_p, P, P, P, I64]),
     "mdx_model_profile_read": (I32, [P, P, I32]),
     "mdx_model_get_policy": (I32, [P, P]),
+    "mdx_linear_workspace_bytes": (I64, [I64, I32, I32, I32]),
+    "mdx_linear": (I32, [P, I64, P, I64, P, P, I64, I64, I32, I32, I32, I32, P, I64, P, I64, P, I64, P]),
+    "mdx_linear_backward_workspace_bytes": (I64, [I64, I32, I32, I32, I32, I32, I32, I32, I32]),
+    "mdx_linear_backward": (I32, [P, I64, P, I64, P, I64, P, I64, I64, I32, I32, I32, I32, P, I64, P, I64, P, P, I64,
+                                  P, I64, P]),
+    "mdx_grouped_linear": (I32, [P, I64, P, P, P, I64, P, I32, I64, I32, I32, I32, I32, P, I64, P, I64, I32, P]),
+    "mdx_grouped_linear_backward_workspace_bytes": (I64, [I32, I64, I32, I32, I32, I32, I32, I32, I32, I32]),
+    "mdx_grouped_linear_backward": (I32, [P, I64, P, I64, P, P, I64, P, I32, I64, I32, I32, I32, I32, P, I64, P, P, P,
+                                          I64, I32, P, I64, P]),
+    "mdx_layer_norm": (I32, [P, I64, P, P, I64, I32, F32, I32, P, I64, P, P, P]),
+    "mdx_layer_norm_backward_workspace_bytes": (I64, [I64, I32, I32]),
+    "mdx_layer_norm_backward": (I32, [P, I64, P, I64, P, P, P, I64, I32, I32, P, I64, P, P, P, I64, P]),
     "mdx_policy_defaults": (I32, [P]),
     "mdx_policy_get": (I32, [P]),
     "mdx_policy_set": (I32, [P]),

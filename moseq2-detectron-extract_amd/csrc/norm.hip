@@ -1,0 +1,453 @@
+// Layer norm over the last axis, forward and backward (include/mdx.h:
+// mdx_layer_norm*).
+//
+//   mean = sum x / D,  rstd = 1 / sqrt(sum (x - mean)^2 / D + eps)
+//   h = (x - mean) rstd,  y = h g + b
+//   dx = rstd (dy g - mean(dy g) - h mean(dy g h)),  dg = sum_rows dy h,  db = sum_rows dy
+//
+// Both are bound by HBM: a row is read once into registers, its sums are taken
+// there in float32 (the variance in a second pass over the registers, around
+// the mean), and the result is written once.  Rows wider than the registers
+// of a workgroup hold are read again instead (k_norm_wide*).
+#include "common.h"
+
+#include <algorithm>
+
+namespace mdx {
+namespace norm {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Un16 { u4 v; };  // rows start anywhere
+template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
+
+template <typename T> struct Piece {
+    union { u4 u; T e[VEC<T>]; };
+};
+// the piece at p, of which the first n elements exist (n <= 0: none); the rest is 0
+template <typename T> __device__ __forceinline__ Piece<T> load(const T *p, int n) {
+    Piece<T> r;
+    if (n >= VEC<T>) {
+        r.u = reinterpret_cast<const Un16<T> *>(p)->v;
+        return r;
+    }
+    r.u = u4{0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < VEC<T>; ++q)
+        if (q < n) r.e[q] = p[q];
+    return r;
+}
+template <typename T> __device__ __forceinline__ void store(T *p, const Piece<T> &v, int n) {
+    if (n >= VEC<T>) {
+        reinterpret_cast<Un16<T> *>(p)->v = v.u;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < VEC<T>; ++q)
+        if (q < n) p[q] = v.e[q];
+}
+
+struct Args {
+    const void *x, *dy;
+    long long ldx, ldy;
+    const float *gamma, *beta;  // [D] or null
+    long long rows;
+    int D;
+    float eps;
+    void *out;                  // y or dx, or null
+    long long ldo;
+    float *mean, *rstd;         // [rows]: written forward (or null), read backward
+    float *part;                // backward: [workgroups][2][D] partial dg, db, or null
+};
+
+// sum over the TPR threads of a row (TPR <= 64: lanes of a wave; above: the
+// workgroup, through LDS).  Every thread gets it.
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float *sh) {
+#pragma unroll
+    for (int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        __syncthreads();  // the sums before this one have been read
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += sh[w];
+    }
+    return v;
+}
+
+// TPR threads hold a row in NP pieces of 16 bytes each
+template <typename T, int TPR, int NP> struct Rows {
+    static constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, V = VEC<T>;
+};
+
+template <typename T, int TPR, int NP>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(Args a) {
+    using L = Rows<T, TPR, NP>;
+    constexpr int V = L::V;
+    __shared__ float sh[16];
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const float inv = 1.f / (float)a.D;
+    float g[NP][V], b[NP][V];
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const int c = (p * TPR + t) * V + q;
+            g[p][q] = a.gamma && c < a.D ? a.gamma[c] : 1.f;
+            b[p][q] = a.beta && c < a.D ? a.beta[c] : 0.f;
+        }
+    for (long long r = (long long)blockIdx.x * L::ROWS + slot; r - slot < a.rows; r += (long long)gridDim.x * L::ROWS) {
+        const bool live = r < a.rows;
+        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.ldx;
+        float v[NP][V], s = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = (p * TPR + t) * V;
+            const Piece<T> w = load(x + c, live ? a.D - c : 0);
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                v[p][q] = (float)w.e[q];
+                s += v[p][q];
+            }
+        }
+        const float mean = row_sum<TPR>(s, sh) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                v[p][q] = (p * TPR + t) * V + q < a.D ? v[p][q] - mean : 0.f;
+                s += v[p][q] * v[p][q];
+            }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(s, sh) * inv + a.eps);
+        if (!live) continue;
+        T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = (p * TPR + t) * V;
+            Piece<T> w;
+#pragma unroll
+            for (int q = 0; q < V; ++q) w.e[q] = (T)(v[p][q] * rstd * g[p][q] + b[p][q]);
+            store(o + c, w, a.D - c);
+        }
+        if (t == 0) {
+            if (a.mean) a.mean[r] = mean;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+    }
+}
+
+// dx, and each workgroup's share of dg and db: a thread keeps the sums of its
+// columns over all rows it takes; the row slots are added through LDS at the end.
+template <typename T, int TPR, int NP>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(Args a) {
+    using L = Rows<T, TPR, NP>;
+    constexpr int V = L::V;
+    __shared__ float sh[16];
+    __shared__ float cols[L::ROWS > 1 ? L::THREADS * NP * V : 1];
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const float inv = 1.f / (float)a.D;
+    float g[NP][V], dg[NP][V], db[NP][V];
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const int c = (p * TPR + t) * V + q;
+            g[p][q] = a.gamma && c < a.D ? a.gamma[c] : 1.f;
+            dg[p][q] = db[p][q] = 0.f;
+        }
+    for (long long r = (long long)blockIdx.x * L::ROWS + slot; r - slot < a.rows; r += (long long)gridDim.x * L::ROWS) {
+        const bool live = r < a.rows;
+        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.ldx;
+        const T *dy = reinterpret_cast<const T *>(a.dy) + (live ? r : 0) * a.ldy;
+        const float mean = live ? a.mean[r] : 0.f, rstd = live ? a.rstd[r] : 0.f;
+        float h[NP][V], d[NP][V], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = (p * TPR + t) * V;
+            const Piece<T> w = load(x + c, live ? a.D - c : 0), y = load(dy + c, live ? a.D - c : 0);
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                const float e = (float)y.e[q];
+                h[p][q] = live && c + q < a.D ? ((float)w.e[q] - mean) * rstd : 0.f;
+                dg[p][q] += e * h[p][q];
+                db[p][q] += e;
+                d[p][q] = e * g[p][q];
+                s1 += d[p][q];
+                s2 += d[p][q] * h[p][q];
+            }
+        }
+        if (!a.out) continue;
+        s1 = row_sum<TPR>(s1, sh) * inv;
+        s2 = row_sum<TPR>(s2, sh) * inv;
+        if (!live) continue;
+        T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = (p * TPR + t) * V;
+            Piece<T> w;
+#pragma unroll
+            for (int q = 0; q < V; ++q) w.e[q] = (T)(rstd * (d[p][q] - s1 - h[p][q] * s2));
+            store(o + c, w, a.D - c);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float *o = a.part + ((long long)blockIdx.x * 2 + k) * a.D;
+        if constexpr (L::ROWS > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int q = 0; q < V; ++q) cols[slot * TPR * NP * V + (p * TPR + t) * V + q] = k ? db[p][q] : dg[p][q];
+            __syncthreads();
+            for (int c = threadIdx.x; c < TPR * NP * V && c < a.D; c += L::THREADS) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < L::ROWS; ++w) v += cols[w * TPR * NP * V + c];
+                o[c] = v;
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int q = 0; q < V; ++q) {
+                    const int c = (p * TPR + t) * V + q;
+                    if (c < a.D) o[c] = k ? db[p][q] : dg[p][q];
+                }
+        }
+    }
+}
+
+// Any width: a workgroup of 1024 reads its row once for each sum and once to write.
+template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide(Args a) {
+    constexpr int V = VEC<T>;
+    __shared__ float sh[16];
+    const long long r = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(a.x) + r * a.ldx;
+    T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
+    float s = 0.f;
+    for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
+        const Piece<T> w = load(x + c, (int)(a.D - c));
+#pragma unroll
+        for (int q = 0; q < V; ++q) s += (float)w.e[q];
+    }
+    const float mean = row_sum<1024>(s, sh) / (float)a.D;
+    s = 0.f;
+    for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
+        const Piece<T> w = load(x + c, (int)(a.D - c));
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            const float d = c + q < a.D ? (float)w.e[q] - mean : 0.f;
+            s += d * d;
+        }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<1024>(s, sh) / (float)a.D + a.eps);
+    for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
+        Piece<T> w = load(x + c, (int)(a.D - c));
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+            if (c + q < a.D)
+                w.e[q] = (T)(((float)w.e[q] - mean) * rstd * (a.gamma ? a.gamma[c + q] : 1.f) +
+                             (a.beta ? a.beta[c + q] : 0.f));
+        store(o + c, w, (int)(a.D - c));
+    }
+    if (threadIdx.x == 0) {
+        if (a.mean) a.mean[r] = mean;
+        if (a.rstd) a.rstd[r] = rstd;
+    }
+}
+template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide_backward(Args a) {
+    constexpr int V = VEC<T>;
+    __shared__ float sh[16];
+    const long long r = blockIdx.x;
+    const T *x = reinterpret_cast<const T *>(a.x) + r * a.ldx, *dy = reinterpret_cast<const T *>(a.dy) + r * a.ldy;
+    T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    float s1 = 0.f, s2 = 0.f;
+    for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
+        const Piece<T> w = load(x + c, (int)(a.D - c)), y = load(dy + c, (int)(a.D - c));
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+            if (c + q < a.D) {
+                const float d = (float)y.e[q] * (a.gamma ? a.gamma[c + q] : 1.f);
+                s1 += d;
+                s2 += d * (((float)w.e[q] - mean) * rstd);
+            }
+    }
+    s1 = row_sum<1024>(s1, sh) / (float)a.D;
+    s2 = row_sum<1024>(s2, sh) / (float)a.D;
+    for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
+        const Piece<T> w = load(x + c, (int)(a.D - c)), y = load(dy + c, (int)(a.D - c));
+        Piece<T> z = w;
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+            if (c + q < a.D) {
+                const float d = (float)y.e[q] * (a.gamma ? a.gamma[c + q] : 1.f), h = ((float)w.e[q] - mean) * rstd;
+                z.e[q] = (T)(rstd * (d - s1 - h * s2));
+            }
+        store(o + c, z, (int)(a.D - c));
+    }
+}
+// dg and db of any width: a workgroup takes 64 columns of one slice of the rows
+template <typename T> __global__ __launch_bounds__(256) void k_norm_wide_sums(Args a) {
+    __shared__ float sh[2][256];
+    const long long c = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const long long per = (a.rows + gridDim.y - 1) / gridDim.y, r1 = min(a.rows, (blockIdx.y + 1) * per);
+    float dg = 0.f, db = 0.f;
+    if (c < a.D)
+        for (long long r = blockIdx.y * per + (threadIdx.x >> 6); r < r1; r += 4) {
+            const float e = (float)reinterpret_cast<const T *>(a.dy)[r * a.ldy + c];
+            dg += e * (((float)reinterpret_cast<const T *>(a.x)[r * a.ldx + c] - a.mean[r]) * a.rstd[r]);
+            db += e;
+        }
+    sh[0][threadIdx.x] = dg;
+    sh[1][threadIdx.x] = db;
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int k = threadIdx.x >> 6, l = threadIdx.x & 63;
+        const float v = sh[k][l] + sh[k][64 + l] + sh[k][128 + l] + sh[k][192 + l];
+        if (c < a.D) a.part[((long long)blockIdx.y * 2 + k) * a.D + c] = v;
+    }
+}
+// dg, db = the workgroups' shares, always added in the same order
+__global__ __launch_bounds__(1024) void k_norm_join(const float *part, int n, int D, float *dg, float *db) {
+    __shared__ float sh[16][64];
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, k = blockIdx.y;
+    const long long c = (long long)blockIdx.x * 64 + l;
+    float *o = k ? db : dg;
+    float v = 0.f;
+    if (c < D)
+        for (int s = w; s < n; s += 16) v += part[((long long)s * 2 + k) * D + c];
+    sh[w][l] = v;
+    __syncthreads();
+    if (w == 0 && c < D && o) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) v += sh[i][l];
+        o[c] = v;
+    }
+}
+
+// ---- host ---------------------------------------------------------------
+// (threads per row, pieces per thread) for D elements: 0 = wider than any
+static int layout(int D, int dtype) {
+    const long long pieces = ((long long)D * (dtype == 0 ? 4 : 2) + 15) / 16;
+    const int cap[] = {16, 32, 64, 128, 256, 512, 1024, 2048};
+    for (int i = 0; i < 8; ++i)
+        if (pieces <= cap[i]) return i + 1;
+    return 0;
+}
+static int rows_per_group(int lay) { return lay == 1 ? 16 : lay == 2 ? 8 : lay <= 5 ? 4 : 1; }
+// workgroups of the backward pass: two on each CU, each with a share of dg and db
+static int backward_groups(long long rows, int D, int dtype) {
+    const int lay = layout(D, dtype);
+    if (!lay) return (int)std::min<long long>(64, std::max<long long>(1, rows / 16));
+    return (int)std::max<long long>(1, std::min<long long>(ceil_div(rows, rows_per_group(lay)), 512));
+}
+
+template <typename T, int TPR, int NP> static void launch(const Args &a, bool back, int groups, hipStream_t s) {
+    using L = Rows<T, TPR, NP>;
+    if (back) {
+        hipLaunchKernelGGL((k_norm_backward<T, TPR, NP>), dim3(groups), dim3(L::THREADS), 0, s, a);
+        return;
+    }
+    const unsigned grid = (unsigned)std::min<long long>(ceil_div(a.rows, L::ROWS), 4096);
+    hipLaunchKernelGGL((k_norm<T, TPR, NP>), dim3(grid), dim3(L::THREADS), 0, s, a);
+}
+template <typename T> static int run(const char *fn, const Args &a, int dtype, bool back, float *dg, float *db,
+                                     hipStream_t s) {
+    const int groups = backward_groups(a.rows, a.D, dtype), lay = layout(a.D, dtype);
+    switch (lay) {
+        case 1: launch<T, 16, 1>(a, back, groups, s); break;
+        case 2: launch<T, 32, 1>(a, back, groups, s); break;
+        case 3: launch<T, 64, 1>(a, back, groups, s); break;
+        case 4: launch<T, 64, 2>(a, back, groups, s); break;
+        case 5: launch<T, 64, 4>(a, back, groups, s); break;
+        case 6: launch<T, 256, 2>(a, back, groups, s); break;
+        case 7: launch<T, 256, 4>(a, back, groups, s); break;
+        case 8: launch<T, 1024, 2>(a, back, groups, s); break;
+        default:
+            if (!back) {
+                hipLaunchKernelGGL(k_norm_wide<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+                break;
+            }
+            // the sums first: dx may be written over dy
+            if (a.part)
+                hipLaunchKernelGGL(k_norm_wide_sums<T>, dim3((unsigned)ceil_div(a.D, 64), groups), dim3(256), 0, s, a);
+            if (a.out && a.rows)
+                hipLaunchKernelGGL(k_norm_wide_backward<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+    }
+    MDX_CHECK_LAUNCH(fn);
+    if (back && a.part) {
+        hipLaunchKernelGGL(k_norm_join, dim3((unsigned)ceil_div(a.D, 64), 2), dim3(1024), 0, s, a.part, groups, a.D, dg,
+                           db);
+        MDX_CHECK_LAUNCH(fn);
+    }
+    return MDX_OK;
+}
+static int dispatch(const char *fn, const Args &a, int dtype, bool back, float *dg, float *db, hipStream_t s) {
+    switch (dtype) {
+        case 0: return run<float>(fn, a, dtype, back, dg, db, s);
+        case 1: return run<_Float16>(fn, a, dtype, back, dg, db, s);
+        default: return run<__bf16>(fn, a, dtype, back, dg, db, s);
+    }
+}
+static int check(const char *fn, int64_t rows, int D, int dtype) {
+    MDX_REQUIRE(dtype == 0 || dtype == 1 || dtype == 3, "%s: dtype must be 0 (f32), 1 (f16) or 3 (bf16)", fn);
+    MDX_REQUIRE(rows >= 0 && D > 0, "%s: bad shape", fn);
+    // a workgroup of 1024 threads for each row there, and fewer than 2^32 threads in a launch
+    MDX_REQUIRE(layout(D, dtype) || rows < (1 << 22), "%s: at most 2^22 - 1 rows of this width", fn);
+    return MDX_OK;
+}
+
+}  // namespace norm
+}  // namespace mdx
+
+using namespace mdx;
+
+extern "C" int mdx_layer_norm(const void *x, int64_t ldx, const float *gamma, const float *beta, int64_t rows, int D,
+                              float eps, int dtype, void *out, int64_t ldo, float *mean, float *rstd,
+                              mdx_stream_t stream) {
+    if (int rc = norm::check("mdx_layer_norm", rows, D, dtype)) return rc;
+    if (rows == 0) return MDX_OK;
+    MDX_REQUIRE(x && out, "mdx_layer_norm: null pointer");
+    MDX_REQUIRE(ldx >= D && ldo >= D, "mdx_layer_norm: a row stride is below its row's length");
+    MDX_REQUIRE(eps >= 0.f, "mdx_layer_norm: eps must not be negative");
+    norm::Args a{};
+    a.x = x; a.ldx = ldx;
+    a.gamma = gamma; a.beta = beta;
+    a.rows = rows; a.D = D; a.eps = eps;
+    a.out = out; a.ldo = ldo;
+    a.mean = mean; a.rstd = rstd;
+    return norm::dispatch("mdx_layer_norm", a, dtype, false, nullptr, nullptr, as_stream(stream));
+}
+
+extern "C" int64_t mdx_layer_norm_backward_workspace_bytes(int64_t rows, int D, int dtype) {
+    if (rows < 0 || D <= 0) return 0;
+    return (int64_t)norm::backward_groups(rows, D, dtype) * 2 * D * 4;
+}
+extern "C" int mdx_layer_norm_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const float *mean,
+                                       const float *rstd, const float *gamma, int64_t rows, int D, int dtype, void *dx,
+                                       int64_t lddx, float *dgamma, float *dbeta, void *workspace,
+                                       int64_t workspace_bytes, mdx_stream_t stream) {
+    if (int rc = norm::check("mdx_layer_norm_backward", rows, D, dtype)) return rc;
+    MDX_REQUIRE(rows == 0 || (grad && x && mean && rstd), "mdx_layer_norm_backward: null pointer");
+    MDX_REQUIRE(ldg >= D && ldx >= D && (!dx || lddx >= D),
+                "mdx_layer_norm_backward: a row stride is below its row's length");
+    const int64_t need = dgamma || dbeta ? mdx_layer_norm_backward_workspace_bytes(rows, D, dtype) : 0;
+    MDX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+                "mdx_layer_norm_backward: needs %lld bytes of workspace, got %lld", (long long)need,
+                (long long)workspace_bytes);
+    if (!need && (!dx || rows == 0)) return MDX_OK;
+    norm::Args a{};
+    a.x = x; a.ldx = ldx;
+    a.dy = grad; a.ldy = ldg;
+    a.gamma = gamma;
+    a.rows = rows; a.D = D;
+    a.out = dx; a.ldo = lddx;
+    a.mean = const_cast<float *>(mean); a.rstd = const_cast<float *>(rstd);
+    a.part = need ? reinterpret_cast<float *>(workspace) : nullptr;
+    return norm::dispatch("mdx_layer_norm_backward", a, dtype, true, dgamma, dbeta, as_stream(stream));
+}
