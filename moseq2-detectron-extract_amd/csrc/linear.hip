@@ -13,6 +13,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace mdx {
 namespace lin {
@@ -67,28 +68,53 @@ template <typename T> __device__ __forceinline__ void store4(T *p, f4 v, int n) 
 }
 
 // ---- activations, in float32 ------------------------------------------------
-constexpr float RSQRT2 = 0.70710678118654752f, RSQRT2PI = 0.39894228040143268f;
-constexpr float TANH_C = 0.79788456080286536f, TANH_A = 0.044715f;
+// On the hardware's exp2 and reciprocal (1 ulp each): with the library's erff,
+// tanhf and division the epilogue of a 256 x 256 tile took longer than its
+// product of 1024 terms.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
+// 1 / (1 + exp(-u))
+__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-u)); }
+// the normal distribution at z: *p its probability (1 + erf(z / sqrt 2)) / 2 by
+// formula 7.1.26 of Abramowitz and Stegun (erf to 1.5e-7), returned
+// exp(-z^2 / 2), which that formula needs and the density is made of
+__device__ __forceinline__ float normal_cdf(float z, float *p) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+    const float e = fast_exp(-x * x);
+    const float c =
+        0.5f * e * t *
+        (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    *p = z < 0.f ? c : 1.f - c;
+    return e;
+}
+// the tanh form: (1 + tanh v) / 2 = logistic(2 v), 2 v = C (z + A z^3)
+constexpr float TANH_C = 1.59576912160573071f, TANH_A = 0.044715f;
 
 __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
         case MDX_ACT_RELU: return z < 0.f ? 0.f : z;  // NaN stays NaN
-        case MDX_ACT_GELU: return 0.5f * z * (1.f + erff(z * RSQRT2));
-        case MDX_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(TANH_C * (z + TANH_A * z * z * z)));
-        case MDX_ACT_SILU: return z / (1.f + expf(-z));
+        case MDX_ACT_GELU: {
+            float p;
+            normal_cdf(z, &p);
+            return z * p;
+        }
+        case MDX_ACT_GELU_TANH: return z * logistic(TANH_C * (z + TANH_A * z * z * z));
+        case MDX_ACT_SILU: return z * logistic(z);
         default: return z;
     }
 }
 __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
-        case MDX_ACT_GELU:
-            return 0.5f * (1.f + erff(z * RSQRT2)) + z * expf(-0.5f * z * z) * RSQRT2PI;
+        case MDX_ACT_GELU: {
+            float p;
+            const float e = normal_cdf(z, &p);
+            return p + z * e * 0.39894228040143268f;
+        }
         case MDX_ACT_GELU_TANH: {
-            const float t = tanhf(TANH_C * (z + TANH_A * z * z * z));
-            return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * TANH_C * (1.f + 3.f * TANH_A * z * z);
+            const float s = logistic(TANH_C * (z + TANH_A * z * z * z));
+            return s + z * s * (1.f - s) * TANH_C * (1.f + 3.f * TANH_A * z * z);
         }
         case MDX_ACT_SILU: {
-            const float s = 1.f / (1.f + expf(-z));
+            const float s = logistic(z);
             return s * (1.f + z * (1.f - s));
         }
         default: return 1.f;
@@ -184,17 +210,97 @@ __device__ __forceinline__ void map_tile(long long id, int ti, int tj, long long
     u = (int)(in / rows);
 }
 
-// bias, residual, activation and the stores of 4 neighbouring outputs
+// N neighbouring values of a row as floats, of which n exist
+template <typename T, int N> __device__ __forceinline__ void load_row(const T *p, int n, float (&v)[N]) {
+    struct __attribute__((packed, aligned(sizeof(T)))) U { T e[N]; };
+    if (n >= N) {
+        const U u = *reinterpret_cast<const U *>(p);
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = (float)u.e[q];
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = q < n ? (float)p[q] : 0.f;
+}
+template <typename T, int N> __device__ __forceinline__ void store_row(T *p, int n, const float (&v)[N]) {
+    struct __attribute__((packed, aligned(sizeof(T)))) U { T e[N]; };
+    if (n >= N) {
+        U u;
+#pragma unroll
+        for (int q = 0; q < N; ++q) u.e[q] = (T)v[q];  // the one rounding to the output's type
+        *reinterpret_cast<U *>(p) = u;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+        if (q < n) p[q] = (T)v[q];
+}
+// bias, residual, activation and the stores of 16 bytes of a row of outputs
 template <typename T>
-__device__ __forceinline__ void finish4(const Args &g, const float *bias, long long i, int j, f4 v) {
+__device__ __forceinline__ void finish(const Args &g, const float *bias, long long i, int j, float (&v)[VEC<T>]) {
+    constexpr int N = VEC<T>;
     const int n = g.J - j;
-    if (bias) v += load4(bias + j, n);
-    if (g.res) v += load4(reinterpret_cast<const T *>(g.res) + i * g.ldr + j, n);
-    if (g.pre) store4(reinterpret_cast<T *>(g.pre) + i * g.ldp + j, v, n);
+    float w[N];
+    if (bias) {
+        load_row<float, N>(bias + j, n, w);
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] += w[q];
+    }
+    if (g.res) {
+        load_row<T, N>(reinterpret_cast<const T *>(g.res) + i * g.ldr + j, n, w);
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] += w[q];
+    }
+    if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i * g.ldp + j, n, v);
     if (g.act != MDX_ACT_NONE)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = act_value(v[q], g.act);
-    store4(reinterpret_cast<T *>(g.out) + i * g.ldo + j, v, n);
+        for (int q = 0; q < N; ++q) v[q] = act_value(v[q], g.act);
+    store_row<T, N>(reinterpret_cast<T *>(g.out) + i * g.ldo + j, n, v);
+}
+
+// A wave's 64 x 64 block of sums, acc(i, j) the 16 x 16 tile of rows 16 i,
+// columns 16 j (lane: row l & 15, columns 4 (l >> 4)..), 32 rows at a time
+// through the wave's own 8.5 KiB of LDS, so that a lane finishes 16 bytes of a
+// row and a row's lanes store a whole line.  The block goes to a slice's
+// partial sums, to zeros (behind the last group) or to the finished outputs.
+constexpr int EPI_PITCH = 68, EPI_BYTES = 32 * EPI_PITCH * 4;
+template <typename T, int MODE, typename F>
+__device__ __forceinline__ void epilogue(const Args &g, const float *bias, bool tail, char *lds, long long row0,
+                                         long long row1, int col0, F acc) {
+    constexpr int N = VEC<T>, PER = 64 / N;  // lanes to a row
+    const int lane = threadIdx.x & 63;
+    float *e = reinterpret_cast<float *>(lds);
+    const long long grp = MODE == GROUP_RED ? blockIdx.z * (long long)g.E + blockIdx.y : blockIdx.z;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f4 *>(e + (16 * i + (lane & 15)) * EPI_PITCH + 16 * j + 4 * (lane >> 4)) =
+                    acc(2 * p + i, j);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll 1
+        for (int k = 0; k < 32 * PER / 64; ++k) {
+            const int r = (64 * k + lane) / PER, c = (64 * k + lane) % PER * N;
+            const long long row = row0 + 32 * p + r;
+            const int col = col0 + c, n = g.J - col;
+            if (row >= row1 || n <= 0) continue;
+            float v[N];
+#pragma unroll
+            for (int q = 0; q < N / 4; ++q)
+                *reinterpret_cast<f4 *>(v + 4 * q) = *reinterpret_cast<const f4 *>(e + r * EPI_PITCH + c + 4 * q);
+            if (g.splits > 1) {
+                store_row<float, N>(g.part + (grp * g.I + row) * g.J + col, n, v);
+            } else if (tail) {
+                store_row<T, N>(reinterpret_cast<T *>(g.out) + row * g.ldo + col, n, v);
+                if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + row * g.ldp + col, n, v);
+            } else {
+                finish<T>(g, bias, row, col, v);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    }
 }
 
 template <typename T> struct Mma;
@@ -291,6 +397,7 @@ __global__ __launch_bounds__(256, 2) void k_product(Args g) {
     using SA = Stage<T, TA>;
     using SB = Stage<T, TB>;
     __shared__ __attribute__((aligned(16))) char lds[2][SA::BYTES + SB::BYTES];
+    static_assert(4 * EPI_BYTES <= sizeof(lds), "the epilogue shares the operands' LDS");
     const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b);
     const float *bias = g.bias;
     long long t;
@@ -365,41 +472,276 @@ __global__ __launch_bounds__(256, 2) void k_product(Args g) {
     }
 
     if (MODE == GROUP_RED) g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
+    __syncthreads();  // the operands' buffers become the epilogue's
+    epilogue<T, MODE>(g, bias, tail, lds[0] + wid * EPI_BYTES, i0 + wi, i1, j0 + wj,
+                      [&](int i, int j) { return acc[i][j]; });
+}
+
+// ---- the large 16-bit tile ----------------------------------------------
+// 256 x 256 outputs per workgroup of 8 waves (one workgroup on a CU), the
+// reduction in K-tiles of 64 through two LDS buffers filled by LDS-DMA.  A
+// K-tile is four half-tiles of 128 rows (B0, A0, B1, A1: 16 KiB each, two
+// 1-KiB DMA instructions of every wave) and four phases, one for each
+// quarter of the outputs: (A0,B0) (A0,B1) (A1,B1) (A1,B0).  A half of A is
+// 128 neighbouring rows, of which wave (g, n) takes rows 64 g..; half h of B is
+// columns 64 n + 32 h .. + 31 of each n, so that a wave's 64 columns lie together.
+//
+// Phase P of a wave is
+//   R(P): LDS reads of one half-tile's fragments, DMA of one half-tile,
+//         waits, barrier
+//   M(P): 16 MFMAs, barrier
+// and the waves of g = 1 run one barrier behind those of g = 0, so that on
+// every SIMD one wave multiplies while the other reads.  Between barriers 2P
+// and 2P + 1 lie R(P) of g = 0 and M(P - 1) of g = 1, then M(P) and R(P).
+//
+// Half-tiles are numbered 4 t + {B0 0, A0 1, B1 2, A1 3}.  R(P) reads number
+// P + 1 (B0 of the next K-tile in the last phase of one: its registers are
+// those of B1, free by then) and issues number P + 8, into the buffer place
+// of number P, whose last read, R(P - 1), both groups have retired (lgkmcnt 0)
+// before the barrier that opens R(P) of g = 0.  Number P + 2, read next, must
+// have landed in every wave before that: each wave lets at most 6 half-tiles
+// (12 instructions) stay outstanding, so a DMA has six phases, about 3000
+// cycles, to arrive, and the queue is never drained before the end.
+//
+// Rows beyond the operand are clamped to its last (their products only reach
+// outputs that are not stored); beyond the reduction's end both operands read
+// zeros, and the K-tiles are rounded up to an even number of at least 4; only
+// the first two and the last two can be partial.
+__device__ __attribute__((aligned(64))) uint4 zero_piece[4];
+
+constexpr int BIG = 256, BIG_BUF = 65536, BIG_LDS = 2 * BIG_BUF, BIG_HALF = 16384;
+
+// Waits and barriers that no memory access is moved across.  The DMA is
+// inline asm, so that the compiler, which would wait for all of it before any
+// LDS read, leaves the count of outstanding ones to these waits.
+template <int VM> __device__ __forceinline__ void big_wait() {  // vmcnt VM, lgkmcnt 0, any expcnt
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | 0x70);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void big_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+// a value that is the same in all lanes, in scalar registers
+__device__ __forceinline__ long long uniform(long long v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (long long)((uint64_t)hi << 32 | lo);
+}
+// 16 bytes a lane from base + off to 1 KiB of LDS at dst (wave-uniform)
+__device__ __forceinline__ void dma16(const void *src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+__device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base)
+                 : "memory");
+}
+
+// a lane's part in staging and reading one operand
+template <typename T, bool TR, bool ISB> struct BigOperand {
+    const char *base;    // first piece of K-tile 0
+    long long step;      // bytes between K-tiles
+    uint32_t off[2][2];  // DMA source of (half, instruction)
+    int r[2];            // reduction index of that piece in its K-tile
+    __device__ __forceinline__ void init(const void *p, long long ld, long long i0, long long I, long long r0, int wid,
+                                         int lane) {
+        base = reinterpret_cast<const char *>(
+            uniform((long long)(reinterpret_cast<uintptr_t>(p) + (TR ? r0 * ld + i0 : i0 * ld + r0) * 2)));
+        step = TR ? 128 * ld : 128;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long row = i0 + wi + 16 * i + (lane & 15);
-        if (row >= i1) continue;
+        for (int d = 0; d < 2; ++d) {
+            const int row = TR ? 4 * (2 * wid + d) + (lane >> 4) : 8 * (2 * wid + d) + (lane >> 3);
+            const int pc = (TR ? lane & 15 : lane & 7) ^ Stage<T, TR>::swz(row);
+            r[d] = TR ? row : 8 * pc;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = j0 + wj + 16 * j + 4 * (lane >> 4);
-            if (col >= g.J) continue;
-            if (g.splits > 1) {
-                const long long grp = MODE == GROUP_RED ? blockIdx.z * (long long)g.E + blockIdx.y : blockIdx.z;
-                store4(g.part + (grp * g.I + row) * g.J + col, acc[i][j], g.J - col);
-            } else if (tail) {
-                store4(reinterpret_cast<T *>(g.out) + row * g.ldo + col, acc[i][j], g.J - col);
-                if (g.pre) store4(reinterpret_cast<T *>(g.pre) + row * g.ldp + col, acc[i][j], g.J - col);
-            } else {
-                finish4<T>(g, bias, row, col, acc[i][j]);
+            for (int h = 0; h < 2; ++h) {
+                const int at = TR ? 8 * pc : row, k = ISB ? 64 * (at >> 5) + 32 * h + (at & 31) : 128 * h + at;
+                const long long i = min(i0 + k, TR ? I - 8 : I - 1);
+                off[h][d] = (uint32_t)(TR ? (row * ld + i - i0) * 2 : (i - i0) * ld * 2 + 16 * pc);
             }
         }
     }
+    // half-tile H of K-tile t
+    template <int H> __device__ __forceinline__ void issue(long long t, uint32_t dst) const {
+#pragma unroll
+        for (int d = 0; d < 2; ++d) dma16s(base + t * step, off[H][d], dst + 1024 * d);
+    }
+    // the same where only `left` elements of the reduction are left from its first on
+    template <int H> __device__ __forceinline__ void issue_part(long long t, long long left, uint32_t dst) const {
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+            dma16(r[d] < left ? base + t * step + off[H][d] : reinterpret_cast<const char *>(zero_piece), dst + 1024 * d);
+    }
+};
+
+template <typename T, bool TA, bool TB, int MODE>
+__global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const char *A = reinterpret_cast<const char *>(g.a), *B = reinterpret_cast<const char *>(g.b);
+    const float *bias = g.bias;
+    long long t;
+    int u;
+    map_tile(blockIdx.x, g.ti, g.tj, t, u);
+    long long i0 = BIG * t, i1 = g.I, r0 = 0, r1 = g.R;
+    const int j0 = BIG * u;
+    bool tail = false;
+    if (MODE == GROUP_ROWS) {
+        const Span s = find_group(g.counts, g.E, g.T, BIG, t, -1);
+        if (s.e < 0 || (s.e == g.E && !g.zero_tail)) return;
+        i0 = s.start + BIG * s.tile;
+        i1 = s.end;
+        if (s.e == g.E) {
+            tail = true;
+        } else {
+            B += s.e * g.gstride * 2;
+            if (bias) bias += (long long)s.e * g.J;
+        }
+    }
+    if (MODE == GROUP_RED) {
+        const Span s = find_group(g.counts, g.E, g.T, 1, 0, blockIdx.y);
+        r0 = s.start;
+        r1 = s.end;
+    }
+    if (g.splits > 1) {
+        const long long steps = (r1 - r0 + 63) / 64, per = (steps + g.splits - 1) / g.splits;
+        r0 = min(r1, r0 + blockIdx.z * per * 64);
+        r1 = min(r1, r0 + per * 64);
+    }
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wid >> 2, wn = wid & 3, f = lane & 15, q = lane >> 4;
+
+    f4 acc[2][2][4][2];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) acc[k >> 4][(k >> 3) & 1][(k >> 1) & 3][k & 1] = f4{0.f, 0.f, 0.f, 0.f};
+
+    if (!tail) {
+        BigOperand<T, TA, false> oa;
+        BigOperand<T, TB, true> ob;
+        oa.init(A, g.lda, i0, i1, r0, wid, lane);
+        ob.init(B, g.ldb, j0, g.J, r0, wid, lane);
+        const long long len = uniform(r1 - r0), KT = max(4ll, (len + 127) / 128 * 2);
+        const uint32_t dst = (uint32_t)(uintptr_t)(lds_s4)lds + 2048u * wid;
+
+        // half-tile Q (B0 A0 B1 A1) of K-tile tt into buffer PAR
+        auto issue = [&](auto Q, auto Par, auto Part, long long tt) {
+            constexpr int n = decltype(Q)::value;
+            const uint32_t d = dst + decltype(Par)::value * BIG_BUF + ((n & 1 ? 0 : 2) + (n >> 1)) * BIG_HALF;
+            if constexpr (decltype(Part)::value) {
+                if constexpr (n & 1)
+                    oa.template issue_part<(n >> 1)>(tt, len - 64 * tt, d);
+                else
+                    ob.template issue_part<(n >> 1)>(tt, len - 64 * tt, d);
+            } else {
+                if constexpr (n & 1)
+                    oa.template issue<(n >> 1)>(tt, d);
+                else
+                    ob.template issue<(n >> 1)>(tt, d);
+            }
+        };
+        // fragments of half-tile h: A0 A1 B0 B1 lie in this order in a buffer
+        u4 fa[2][4], fx[2][2], fy[2][2];
+        auto read_a = [&](int h, int par) {
+            const char *p = lds + par * BIG_BUF + h * BIG_HALF;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) fa[s][i] = Stage<T, TA>::frag(p, 64 * grp + 16 * i, s);
+        };
+        auto read_b = [&](u4 (&fb)[2][2], int h, int par) {
+            const char *p = lds + par * BIG_BUF + (2 + h) * BIG_HALF;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) fb[s][j] = Stage<T, TB>::frag(p, 32 * wn + 16 * j, s);
+        };
+        auto mul = [&](f4 (&c)[4][2], const u4 (&fb)[2][2]) {
+            big_barrier();
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) c[i][j] = Mma<T>::mul(fb[s][j], fa[s][i], c[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            big_barrier();
+        };
+        using std::integral_constant;
+        constexpr integral_constant<int, 0> c0{};
+        constexpr integral_constant<int, 1> c1{};
+        constexpr integral_constant<int, 2> c2{};
+        constexpr integral_constant<int, 3> c3{};
+        // one K-tile in buffer PAR; END: 0 and 3 issue K-tile tt + 2 (3: which
+        // may be partial), 1 and 2 are the last two
+        auto tile = [&](auto End, auto Par, long long tt, u4 (&x)[2][2], u4 (&y)[2][2]) {
+            constexpr int END = decltype(End)::value, PAR = decltype(Par)::value;
+            constexpr bool MORE = END == 0 || END == 3;
+            constexpr integral_constant<int, END == 3> part{};
+            read_a(0, PAR);
+            if constexpr (MORE) issue(c0, Par, part, tt + 2);
+            big_wait<MORE ? 12 : END == 1 ? 10 : 2>();
+            mul(acc[0][0], x);
+            read_b(y, 1, PAR);
+            if constexpr (MORE) issue(c1, Par, part, tt + 2);
+            big_wait<MORE ? 12 : END == 1 ? 8 : 0>();
+            mul(acc[0][1], y);
+            read_a(1, PAR);
+            if constexpr (MORE) issue(c2, Par, part, tt + 2);
+            big_wait<MORE ? 12 : END == 1 ? 6 : 0>();
+            mul(acc[1][1], y);
+            if constexpr (END != 2) read_b(y, 0, 1 - PAR);
+            if constexpr (MORE) issue(c3, Par, part, tt + 2);
+            big_wait<MORE ? 12 : END == 1 ? 4 : 0>();
+            mul(acc[1][0], x);
+        };
+        issue(c0, c0, c1, 0); issue(c1, c0, c1, 0); issue(c2, c0, c1, 0); issue(c3, c0, c1, 0);
+        issue(c0, c1, c1, 1); issue(c1, c1, c1, 1); issue(c2, c1, c1, 1); issue(c3, c1, c1, 1);
+        big_wait<12>();
+        big_barrier();
+        read_b(fx, 0, 0);
+        big_wait<12>();
+        big_barrier();
+        if (grp == 1) big_barrier();  // one behind
+        for (long long tt = 0; tt < KT - 4; tt += 2) {
+            tile(c0, c0, tt, fx, fy);
+            tile(c0, c1, tt + 1, fy, fx);
+        }
+        tile(c3, c0, KT - 4, fx, fy);
+        tile(c3, c1, KT - 3, fy, fx);
+        tile(c1, c0, KT - 2, fx, fy);
+        tile(c2, c1, KT - 1, fy, fx);
+        if (grp == 0) big_barrier();  // every wave crosses as many
+    }
+
+    if (MODE == GROUP_RED) g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
+    __syncthreads();  // the operands' buffers become the epilogue's
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi)
+        epilogue<T, MODE>(g, bias, tail, lds + wid * EPI_BYTES, i0 + 128 * hi + 64 * grp, i1, j0 + 64 * wn,
+                          [&](int i, int j) { return acc[hi][j >> 1][i][j & 1]; });
 }
 
 // The slices' partial sums, added in their order (no atomics: the same result
-// on every call), and the epilogue; one thread per 4 outputs.
+// on every call), and the epilogue; one thread per 16 bytes of output.
 template <typename T>
 __global__ __launch_bounds__(256) void k_product_join(Args g) {
-    const long long quads = (g.J + 3) / 4, id = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= g.I * quads) return;
-    const long long row = id / quads;
-    const int col = (int)(id - row * quads) * 4;
+    constexpr int N = VEC<T>;
+    const long long per = (g.J + N - 1) / N, id = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= g.I * per) return;
+    const long long row = id / per;
+    const int col = (int)(id - row * per) * N;
     const long long E = gridDim.y;
-    f4 v{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < g.splits; ++s)
-        v += load4(g.part + ((s * E + blockIdx.y) * g.I + row) * g.J + col, g.J - col);
+    float v[N] = {}, w[N];
+    for (int s = 0; s < g.splits; ++s) {
+        load_row<float, N>(g.part + ((s * E + blockIdx.y) * g.I + row) * g.J + col, g.J - col, w);
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] += w[q];
+    }
     g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
-    finish4<T>(g, g.bias, row, col, v);
+    finish<T>(g, g.bias, row, col, v);
 }
 
 // dz = dy act'(z) in T, and the column sums of dz before that rounding.  A
@@ -485,18 +827,41 @@ static int act_slices(int E, long long T, int N) {
     return (int)std::max<long long>(1, std::min<long long>(want, (T / std::max(E, 1) + 31) / 32));
 }
 
+// the large tile: both operands in whole aligned pieces of 16 bytes, and
+// enough tiles
+template <typename T, bool TA, bool TB> static bool use_big(const Args &g, int mode) {
+    if (sizeof(T) != 2) return false;
+    auto piece = [](const void *p, long long ld) {
+        return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(2 * ld)) % 16 == 0 && ld < (1ll << 22);
+    };
+    if (!piece(g.a, g.lda) || !piece(g.b, g.ldb) || g.gstride % 8) return false;
+    if ((TA ? g.I : g.R) % 8 || (TB ? g.J : g.R) % 8) return false;
+    const long long groups = mode == GROUP_RED ? g.E : 1;
+    return ceil_div(g.I, BIG) * ceil_div(g.J, BIG) * groups * g.splits >= 128;
+}
+
 template <typename T, bool TA, bool TB, int MODE> static int launch_product(Args g, hipStream_t s) {
+    const bool big = use_big<T, TA, TB>(g, MODE);
+    const int side = big ? BIG : 128, threads = big ? 512 : 256;
     const long long bound = MODE == GROUP_ROWS ? g.E + 1 : 0;  // one partial tile more for each group
-    const long long ti = ceil128(g.I) + bound, tj = ceil128(g.J);
-    MDX_REQUIRE(ti * tj < (1ll << 24), "mdx_linear: too many output tiles");  // 2^32 threads
+    const long long ti = ceil_div(g.I, side) + bound, tj = ceil_div(g.J, side);
+    MDX_REQUIRE(ti * tj * threads < (1ll << 32), "mdx_linear: too many output tiles");
     g.ti = (int)ti;
     g.tj = (int)tj;
     const dim3 grid((unsigned)(ti * tj), MODE == GROUP_RED ? g.E : 1, g.splits);
-    hipLaunchKernelGGL((k_product<T, TA, TB, MODE>), grid, dim3(256), 0, s, g);
+    if constexpr (sizeof(T) == 2) {
+        if (big) {
+            static const hipError_t attr = hipFuncSetAttribute(
+                reinterpret_cast<const void *>(k_product_big<T, TA, TB, MODE>),
+                hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
+            MDX_HIP(attr);
+            hipLaunchKernelGGL((k_product_big<T, TA, TB, MODE>), grid, dim3(512), BIG_LDS, s, g);
+        }
+    }
+    if (!big) hipLaunchKernelGGL((k_product<T, TA, TB, MODE>), grid, dim3(256), 0, s, g);
     MDX_CHECK_LAUNCH("mdx_linear");
     if (g.splits > 1) {
-        const long long quads = (g.J + 3) / 4;
-        const dim3 jg((unsigned)ceil_div(g.I * quads, 256), MODE == GROUP_RED ? g.E : 1);
+        const dim3 jg((unsigned)ceil_div(g.I * ceil_div(g.J, VEC<T>), 256), MODE == GROUP_RED ? g.E : 1);
         hipLaunchKernelGGL(k_product_join<T>, jg, dim3(256), 0, s, g);
         MDX_CHECK_LAUNCH("mdx_linear");
     }
