@@ -28,45 +28,61 @@ typedef __attribute__((address_space(3))) s4 *lds_s4;
 // rows start at any element: vector accesses of the element's alignment
 // (global_load_dwordx4 takes any address in the unaligned access mode of HSA)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Un16 { u4 v; };
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Un4 { T v[4]; };
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 
-// 16 bytes of a row, of which the first n elements exist (n <= 0: none)
-template <typename T> __device__ __forceinline__ u4 load_piece(const T *p, long long n) {
-    if (n >= VEC<T>) return reinterpret_cast<const Un16<T> *>(p)->v;
-    union { u4 u; T e[VEC<T>]; } r;
+// 16 bytes of a row from its element c on, of which the first n exist (n <= 0:
+// none); the rest is zero.  The last piece of a row is read as the 16 bytes
+// that end with it, shifted down.
+template <typename T> __device__ __forceinline__ u4 load_piece(const T *p, long long c, long long n) {
+    constexpr int N = VEC<T>;
+    if (n >= N) return reinterpret_cast<const Un16<T> *>(p)->v;
+    union { u4 u; unsigned long long d[2]; T e[N]; } r;
     r.u = u4{0, 0, 0, 0};
+    if (n <= 0) return r.u;
+    if (c + n >= N) {
+        r.u = reinterpret_cast<const Un16<T> *>(p - (N - n))->v;
+        int s = (int)(N - n) * 8 * (int)sizeof(T);
+        if (s >= 64) {
+            r.d[0] = r.d[1];
+            r.d[1] = 0;
+            s -= 64;
+        }
+        if (s) {
+            r.d[0] = r.d[0] >> s | r.d[1] << (64 - s);
+            r.d[1] >>= s;
+        }
+        return r.u;
+    }
 #pragma unroll
-    for (int q = 0; q < VEC<T>; ++q)
+    for (int q = 0; q < N; ++q)
         if (q < n) r.e[q] = p[q];
     return r.u;
 }
-template <typename T> __device__ __forceinline__ f4 load4(const T *p, int n) {
-    if (n >= 4) {
-        const Un4<T> v = *reinterpret_cast<const Un4<T> *>(p);
-        return f4{(float)v.v[0], (float)v.v[1], (float)v.v[2], (float)v.v[3]};
+// N values of a row from its element c on as floats, of which the first n exist
+template <typename T, int N> __device__ __forceinline__ void load_row(const T *p, int c, int n, float (&v)[N]) {
+    constexpr int P = VEC<T>;
+#pragma unroll
+    for (int k = 0; k < N / P; ++k) {
+        union { u4 u; T e[P]; } r;
+        r.u = load_piece(p + k * P, c + k * P, n - k * P);
+#pragma unroll
+        for (int q = 0; q < P; ++q) v[k * P + q] = (float)r.e[q];
     }
-    f4 r{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int q = 0; q < 3; ++q)
-        if (q < n) r[q] = (float)p[q];
-    return r;
 }
-// one rounding to the output's type
-template <typename T> __device__ __forceinline__ void store4(T *p, f4 v, int n) {
-    if (n >= 4) {
-        Un4<T> o;
+template <typename T, int N> __device__ __forceinline__ void store_row(T *p, int n, const float (&v)[N]) {
+    struct __attribute__((packed, aligned(sizeof(T)))) U { T e[N]; };
+    if (n >= N) {
+        U u;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o.v[q] = (T)v[q];
-        *reinterpret_cast<Un4<T> *>(p) = o;
+        for (int q = 0; q < N; ++q) u.e[q] = (T)v[q];  // the one rounding to the output's type
+        *reinterpret_cast<U *>(p) = u;
         return;
     }
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
+    for (int q = 0; q < N; ++q)
         if (q < n) p[q] = (T)v[q];
 }
-
 // ---- activations, in float32 ------------------------------------------------
 // On the hardware's exp2 and reciprocal (1 ulp each): with the library's erff,
 // tanhf and division the epilogue of a 256 x 256 tile took longer than its
@@ -154,150 +170,256 @@ struct Args {
 
 enum { DENSE = 0, GROUP_ROWS = 1, GROUP_RED = 2 };
 
+// a value that is the same in all lanes, and lane l's value, in scalar registers
+__device__ __forceinline__ long long uniform(long long v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+    return (long long)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
+}
+__device__ __forceinline__ long long lane_value(long long v, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l);
+    return (long long)((uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32 | lo);
+}
+
 struct Span {
     int e;                 // group, E = the rows behind the last one, -1 = none
     long long start, end;  // its rows
-    long long tile;        // tile within the group
+    long long tile, tile0; // tile within the group; the group's first tile
 };
 
-// The group holding output tile `tile` when each group's rows are cut into
-// tiles of bm (want < 0), or group `want` itself.  Every wave scans the counts 64 at a
-// time with its lanes, so no pass over the counts has to run before.
+// The group holding tile `tile` when each group's rows are cut into tiles of
+// bm (want < 0), or group `want` itself (E: the rows behind the last one).
+// Every wave scans the counts 64 at a time with its lanes, so no pass over the
+// counts has to run before.
 __device__ __forceinline__ Span find_group(const int *counts, int E, long long T, int bm, long long tile, int want) {
     const int lane = threadIdx.x & 63;
     long long row0 = 0, tile0 = 0;
     for (int base = 0; base < E; base += 64) {
-        long long c = base + lane < E ? max(counts[base + lane], 0) : 0;
+        const long long c = base + lane < E ? max(counts[base + lane], 0) : 0;
         long long rows = c;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const long long v = __shfl_up(rows, d);
             if (lane >= d) rows += v;
         }
-        const long long s = min(row0 + rows - c, T), e = min(row0 + rows, T);
-        const long long mine = want >= 0 ? 0 : (e - s + bm - 1) / bm;
+        const long long s = min(row0 + rows - c, T), e = min(row0 + rows, T), mine = (e - s + bm - 1) / bm;
         long long tiles = mine;
-        if (want < 0) {
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const long long v = __shfl_up(tiles, d);
-                if (lane >= d) tiles += v;
-            }
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long v = __shfl_up(tiles, d);
+            if (lane >= d) tiles += v;
         }
         const long long t1 = tile0 + tiles, t0 = t1 - mine;
         const unsigned long long hit =
             __ballot(base + lane < E && (want >= 0 ? base + lane == want : tile >= t0 && tile < t1));
         if (hit) {
             const int l = __ffsll(hit) - 1;
-            return Span{base + l, __shfl(s, l), __shfl(e, l), tile - __shfl(t0, l)};
+            const long long first = lane_value(t0, l);
+            return Span{base + l, lane_value(s, l), lane_value(e, l), tile - first, first};
         }
-        row0 = min(row0 + __shfl(rows, 63), T);
-        tile0 = __shfl(t1, 63);
+        row0 = min(row0 + lane_value(rows, 63), T);
+        tile0 = lane_value(t1, 63);
     }
     if (want >= 0 ? want == E : row0 < T && tile < tile0 + (T - row0 + bm - 1) / bm)
-        return Span{E, row0, T, tile - tile0};
-    return Span{-1, 0, 0, 0};
+        return Span{E, row0, T, tile - tile0, tile0};
+    return Span{-1, 0, 0, 0, 0};
 }
 
-// workgroup -> tile: contiguous ranges of tiles for each of the 8 XCDs (their
-// L2s are separate), and in a range squares of 8 row tiles, column by column
-__device__ __forceinline__ void map_tile(long long id, int ti, int tj, long long &t, int &u) {
-    const long long n = (long long)ti * tj, q = n / 8, r = n % 8, x = id % 8;
+// tiles of bm rows of all groups; *rows: the rows that they hold together
+__device__ __forceinline__ long long count_tiles(const int *counts, int E, long long T, int bm, long long *rows) {
+    const int lane = threadIdx.x & 63;
+    long long row0 = 0, n = 0;
+    for (int base = 0; base < E; base += 64) {
+        const long long c = base + lane < E ? max(counts[base + lane], 0) : 0;
+        long long r = c;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long v = __shfl_up(r, d);
+            if (lane >= d) r += v;
+        }
+        long long mine = (min(row0 + r, T) - min(row0 + r - c, T) + bm - 1) / bm;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
+        n += uniform(mine);
+        row0 = min(row0 + lane_value(r, 63), T);
+    }
+    *rows = row0;
+    return n;
+}
+
+// tile id of ti x tj -> (row tile, column tile): contiguous ranges of tiles for
+// each of the 8 XCDs (their L2s are separate; workgroups go to them in turn),
+// and in a range squares of 8 row tiles, column by column
+__device__ __forceinline__ void map_tile(unsigned id, unsigned ti, unsigned tj, int &t, int &u) {
+    const unsigned n = ti * tj, q = n / 8, r = n % 8, x = id % 8;
     id = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + id / 8;
-    const long long per = 8ll * tj, g = id / per, in = id - g * per;
-    const int rows = (int)min(8ll, ti - 8 * g);
+    const unsigned per = 8 * tj, g = id / per, in = id - g * per, rows = min(8u, ti - 8 * g);
     t = 8 * g + in % rows;
-    u = (int)(in / rows);
+    u = in / rows;
 }
 
-// N neighbouring values of a row as floats, of which n exist
-template <typename T, int N> __device__ __forceinline__ void load_row(const T *p, int n, float (&v)[N]) {
-    struct __attribute__((packed, aligned(sizeof(T)))) U { T e[N]; };
-    if (n >= N) {
-        const U u = *reinterpret_cast<const U *>(p);
-#pragma unroll
-        for (int q = 0; q < N; ++q) v[q] = (float)u.e[q];
-        return;
+// the tiles of a product: ids 0 .. n - 1
+struct Work {
+    int n, ti;       // row tiles that hold rows
+    long long rows;  // grouped rows: rows of all groups
+};
+template <int MODE> __device__ __forceinline__ Work list_work(const Args &g, int bi) {
+    Work k{g.ti * g.tj * g.splits, g.ti, g.I};
+    if (MODE == GROUP_RED) k.n *= g.E;
+    if (MODE == GROUP_ROWS) {  // g.ti is a bound
+        k.ti = (int)count_tiles(g.counts, g.E, g.T, bi, &k.rows);
+        k.n = (k.ti + (g.zero_tail ? (int)((g.T - k.rows + bi - 1) / bi) : 0)) * g.tj;
     }
-#pragma unroll
-    for (int q = 0; q < N; ++q) v[q] = q < n ? (float)p[q] : 0.f;
+    return k;
 }
-template <typename T, int N> __device__ __forceinline__ void store_row(T *p, int n, const float (&v)[N]) {
-    struct __attribute__((packed, aligned(sizeof(T)))) U { T e[N]; };
-    if (n >= N) {
-        U u;
-#pragma unroll
-        for (int q = 0; q < N; ++q) u.e[q] = (T)v[q];  // the one rounding to the output's type
-        *reinterpret_cast<U *>(p) = u;
-        return;
+// One of them: rows i0 .. of i1, columns from j0, the reduction r0 .. r1, and
+// the offsets of its group and slice.
+struct Where {
+    long long i0, i1, r0, r1, boff, biasoff, ooff;
+    int j0, grp;  // grp: place of its partial sums
+    bool tail;    // rows behind the last group: zeros
+};
+template <int MODE>
+__device__ __forceinline__ Where locate(const Args &g, const Work &k, int id, int bi, int bj, int bk) {
+    Where w{0, g.I, 0, g.R, 0, 0, 0, 0, 0, false};
+    int t, u;
+    if (MODE == GROUP_ROWS && id >= k.ti * g.tj) {  // the rows behind come last, so that the XCDs' ranges are even
+        id -= k.ti * g.tj;
+        w.i0 = k.rows + (long long)(id / g.tj) * bi;
+        w.i1 = g.T;
+        w.j0 = id % g.tj * bj;
+        w.r1 = 0;
+        w.tail = true;
+        return w;
     }
-#pragma unroll
-    for (int q = 0; q < N; ++q)
-        if (q < n) p[q] = (T)v[q];
+    int e = 0, z = 0;
+    if (MODE == GROUP_RED || g.splits > 1) {
+        const int per = g.ti * g.tj;
+        w.grp = id / per;
+        id -= w.grp * per;
+        z = w.grp;
+        if (MODE == GROUP_RED) {
+            z = w.grp / g.E;
+            e = w.grp - z * g.E;
+        }
+    }
+    map_tile(id, k.ti, g.tj, t, u);
+    w.i0 = (long long)bi * t;
+    w.j0 = bj * u;
+    if (MODE == GROUP_ROWS) {
+        const Span s = find_group(g.counts, g.E, g.T, bi, t, -1);
+        w.i0 = s.start + bi * s.tile;
+        w.i1 = s.end;
+        w.boff = s.e * g.gstride;
+        w.biasoff = (long long)s.e * g.J;
+    }
+    if (MODE == GROUP_RED) {
+        const Span s = find_group(g.counts, g.E, g.T, 1, 0, e);
+        w.r0 = s.start;
+        w.r1 = s.end;
+        w.ooff = e * g.gstride;
+    }
+    if (g.splits > 1) {  // this slice of the reduction, in whole steps
+        const int steps = (int)((w.r1 - w.r0 + bk - 1) / bk), per = (steps + g.splits - 1) / g.splits;
+        w.r0 = min(w.r1, w.r0 + (long long)z * per * bk);
+        w.r1 = min(w.r1, w.r0 + (long long)per * bk);
+    }
+    return w;
 }
-// bias, residual, activation and the stores of 16 bytes of a row of outputs
+
+// 16 bytes of a row of outputs from their sums v: bias b (zeros if there is
+// none), residual, activation and the stores
 template <typename T>
-__device__ __forceinline__ void finish(const Args &g, const float *bias, long long i, int j, float (&v)[VEC<T>]) {
+__device__ __forceinline__ void finish(const Args &g, long long ooff, long long i, int j, float (&v)[VEC<T>],
+                                       const float (&b)[VEC<T>], u4 res) {
     constexpr int N = VEC<T>;
     const int n = g.J - j;
-    float w[N];
-    if (bias) {
-        load_row<float, N>(bias + j, n, w);
+    union { u4 u; T e[N]; } r;
+    r.u = res;
+    if (g.bias)
 #pragma unroll
-        for (int q = 0; q < N; ++q) v[q] += w[q];
-    }
-    if (g.res) {
-        load_row<T, N>(reinterpret_cast<const T *>(g.res) + i * g.ldr + j, n, w);
+        for (int q = 0; q < N; ++q) v[q] += b[q];
+    if (g.res)
 #pragma unroll
-        for (int q = 0; q < N; ++q) v[q] += w[q];
-    }
+        for (int q = 0; q < N; ++q) v[q] += (float)r.e[q];
     if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i * g.ldp + j, n, v);
     if (g.act != MDX_ACT_NONE)
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] = act_value(v[q], g.act);
-    store_row<T, N>(reinterpret_cast<T *>(g.out) + i * g.ldo + j, n, v);
+    store_row<T, N>(reinterpret_cast<T *>(g.out) + ooff + i * g.ldo + j, n, v);
 }
-
-// A wave's 64 x 64 block of sums, acc(i, j) the 16 x 16 tile of rows 16 i,
-// columns 16 j (lane: row l & 15, columns 4 (l >> 4)..), 32 rows at a time
-// through the wave's own 8.5 KiB of LDS, so that a lane finishes 16 bytes of a
-// row and a row's lanes store a whole line.  The block goes to a slice's
-// partial sums, to zeros (behind the last group) or to the finished outputs.
-constexpr int EPI_PITCH = 68, EPI_BYTES = 32 * EPI_PITCH * 4;
-template <typename T, int MODE, typename F>
-__device__ __forceinline__ void epilogue(const Args &g, const float *bias, bool tail, char *lds, long long row0,
-                                         long long row1, int col0, F acc) {
-    constexpr int N = VEC<T>, PER = 64 / N;  // lanes to a row
-    const int lane = threadIdx.x & 63;
+template <typename T> __device__ __forceinline__ u4 load_residual(const Args &g, long long i, int j) {
+    return g.res ? load_piece(reinterpret_cast<const T *>(g.res) + i * g.ldr + j, j, g.J - j) : u4{0, 0, 0, 0};
+}
+// where the sums go: a slice's partial sums, zeros behind the last group, or
+// the finished outputs
+template <typename T>
+__device__ __forceinline__ void store_outputs(const Args &g, const Where &w, long long row, int col,
+                                              float (&v)[VEC<T>], const float (&b)[VEC<T>], u4 res) {
+    constexpr int N = VEC<T>;
+    const int n = g.J - col;
+    if (g.splits > 1) {
+        store_row<float, N>(g.part + (w.grp * g.I + row) * g.J + col, n, v);
+    } else if (w.tail) {
+        store_row<T, N>(reinterpret_cast<T *>(g.out) + row * g.ldo + col, n, v);
+        if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + row * g.ldp + col, n, v);
+    } else {
+        finish<T>(g, w.ooff, row, col, v, b, res);
+    }
+}
+// A wave's sums, P blocks of 16 rows by Q columns (64 or 32) from column col0
+// on: block p, whose first row is row(p), is put by put(p, e) into the wave's
+// own epi_bytes(Q) of LDS e and from there finished, 16 bytes of a row to a
+// lane, so that a row's lanes store whole lines.  A lane's column is the same
+// in all blocks: its bias is loaded once, and the residual a block ahead.
+// put_block is a 16 x 16 tile's part: lane (row l & 15, columns 4 (l >> 4)..);
+// slots of 16 bytes are XOR-swizzled by row against bank conflicts.
+template <int N, int K = 0, typename F> __device__ __forceinline__ void static_for(F f) {
+    if constexpr (K < N) {
+        f(std::integral_constant<int, K>{});
+        static_for<N, K + 1>(f);
+    }
+}
+constexpr int epi_bytes(int q) { return 16 * q * 4; }
+template <int Q> __device__ __forceinline__ void put_block(float *e, int j, f4 v) {
+    const int lane = threadIdx.x & 63, r = lane & 15, slot = (4 * j + (lane >> 4)) ^ (r & (Q / 4 - 1));
+    *reinterpret_cast<f4 *>(e + r * Q + 4 * slot) = v;
+}
+template <typename T, int Q, int P, typename R, typename F>
+__device__ __forceinline__ void epilogue(const Args &g, const Where &w, char *lds, int col0, R row, F put) {
+    constexpr int N = VEC<T>, PER = Q / N, K = 16 * PER / 64;  // PER lanes to a row, K pieces to a lane
+    const int lane = threadIdx.x & 63, c = lane % PER * N, col = col0 + c;
     float *e = reinterpret_cast<float *>(lds);
-    const long long grp = MODE == GROUP_RED ? blockIdx.z * (long long)g.E + blockIdx.y : blockIdx.z;
+    const bool in = col < g.J, plain = g.splits == 1 && !w.tail;
+    float b[N] = {};
+    if (g.bias && plain) load_row<float, N>(g.bias + w.biasoff + col, col, in ? g.J - col : 0, b);
+    u4 next[K];
+    auto prefetch = [&](int p) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<f4 *>(e + (16 * i + (lane & 15)) * EPI_PITCH + 16 * j + 4 * (lane >> 4)) =
-                    acc(2 * p + i, j);
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        for (int k = 0; k < K; ++k) {
+            const long long i = row(p) + (64 * k + lane) / PER;
+            next[k] = plain && in && i < w.i1 ? load_residual<T>(g, i, col) : u4{0, 0, 0, 0};
+        }
+    };
+    prefetch(0);
 #pragma unroll 1
-        for (int k = 0; k < 32 * PER / 64; ++k) {
-            const int r = (64 * k + lane) / PER, c = (64 * k + lane) % PER * N;
-            const long long row = row0 + 32 * p + r;
-            const int col = col0 + c, n = g.J - col;
-            if (row >= row1 || n <= 0) continue;
+    for (int p = 0; p < P; ++p) {
+        put(p, e);
+        u4 res[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) res[k] = next[k];
+        if (p + 1 < P) prefetch(p + 1);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int r = (64 * k + lane) / PER;
+            const long long i = row(p) + r;
+            if (i >= w.i1 || !in) continue;
             float v[N];
 #pragma unroll
             for (int q = 0; q < N / 4; ++q)
-                *reinterpret_cast<f4 *>(v + 4 * q) = *reinterpret_cast<const f4 *>(e + r * EPI_PITCH + c + 4 * q);
-            if (g.splits > 1) {
-                store_row<float, N>(g.part + (grp * g.I + row) * g.J + col, n, v);
-            } else if (tail) {
-                store_row<T, N>(reinterpret_cast<T *>(g.out) + row * g.ldo + col, n, v);
-                if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + row * g.ldp + col, n, v);
-            } else {
-                finish<T>(g, bias, row, col, v);
-            }
+                *reinterpret_cast<f4 *>(v + 4 * q) =
+                    *reinterpret_cast<const f4 *>(e + r * Q + 4 * ((c / 4 + q) ^ (r & (Q / 4 - 1))));
+            store_outputs<T>(g, w, i, col, v, b, res[k]);
         }
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     }
@@ -325,40 +447,42 @@ template <> struct Mma<float> {
     }
 };
 
-// 128 rows (i) of an operand by 128 bytes of reduction, staged in LDS.
-// TR = 0: [128][128 B], 16-B pieces XOR-swizzled by row; a fragment (row
+// SIDE rows (i) of an operand by 128 bytes of reduction, staged in LDS.
+// TR = 0: [SIDE][128 B], 16-B pieces XOR-swizzled by row; a fragment (row
 // l & 15, piece 4 s + (l >> 4)) is one b128 read.
-// TR = 1: [128 B / sizeof(T)][128]; 16-bit fragments are two transposing
+// TR = 1: [128 B / sizeof(T)][SIDE]; 16-bit fragments are two transposing
 // 64-bit reads (16 lanes give the addresses of a 4 x 16 block, lane i gets
 // its column i), 32-bit ones four b32 reads.  The swizzle spreads the rows
 // that one read takes over all banks.
-template <typename T, bool TR> struct Stage {
+template <typename T, bool TR, int SIDE> struct Stage {
     static constexpr int BK = 128 / (int)sizeof(T);
-    static constexpr int BYTES = 128 * 128;
-    static constexpr int PITCH = TR ? 128 * (int)sizeof(T) : 128;
+    static constexpr int BYTES = SIDE * 128;
+    static constexpr int PITCH = TR ? SIDE * (int)sizeof(T) : 128;
     static constexpr int PPR = PITCH / 16;           // pieces per stored row
-    static constexpr int STEP = 256 / PPR;           // rows between a thread's four pieces
+    static constexpr int STEP = 256 / PPR;           // rows between a thread's pieces
+    static constexpr int N = SIDE / 32;              // pieces of each of 256 threads
 
     static __device__ __forceinline__ int swz(int row) {
         if (!TR) return (row >> 1) & 7;
-        if (sizeof(T) == 2) return ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
-        return ((row >> 2) & 3) << 2;
+        if (sizeof(T) == 4) return ((row >> 2) & 3) << 2;
+        if (SIDE == 64) return (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) << 1;  // two rows to all banks
+        return ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
     }
-    // the thread's four pieces of the tile whose first i is i0 and first r is r0
+    // the thread's pieces of the tile whose first i is i0 and first r is r0
     static __device__ __forceinline__ void load(const T *p, long long ld, long long i0, long long I, long long r0,
-                                                long long R, u4 (&v)[4]) {
+                                                long long R, u4 (&v)[N]) {
         const int pc = threadIdx.x % PPR, row = threadIdx.x / PPR;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < N; ++q) {
             const long long w = (TR ? r0 : i0) + row + STEP * q, c = (TR ? i0 : r0) + pc * VEC<T>;
             const long long left = w < (TR ? R : I) ? (TR ? I : R) - c : 0;
-            v[q] = load_piece(left > 0 ? p + w * ld + c : p, left);
+            v[q] = load_piece(left > 0 ? p + w * ld + c : p, c, left);
         }
     }
-    static __device__ __forceinline__ void write(char *lds, const u4 (&v)[4]) {
+    static __device__ __forceinline__ void write(char *lds, const u4 (&v)[N]) {
         const int pc = threadIdx.x % PPR, row = threadIdx.x / PPR;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < N; ++q) {
             const int r = row + STEP * q;
             *reinterpret_cast<u4 *>(lds + r * PITCH + ((pc ^ swz(r)) << 4)) = v[q];
         }
@@ -387,94 +511,141 @@ template <typename T, bool TR> struct Stage {
     }
 };
 
-// Tile 128 x 128 per workgroup of 4 waves, each 64 x 64 of 16 x 16 MFMA tiles;
-// the reduction in steps of 128 bytes through two LDS buffers, the next step's
-// global loads in flight in registers meanwhile.  B is the MFMA's first
-// operand, so a lane ends with 4 neighbouring columns of one row.
+// Tile SIDE x SIDE (128 or 64) per workgroup of 4 waves, each a quarter of 16 x
+// 16 MFMA tiles; the reduction in steps of 128 bytes through two LDS buffers,
+// the next step's global loads in flight in registers meanwhile.  B is the
+// MFMA's first operand, so a lane ends with 4 neighbouring columns of one row.
 // Any alignment, any sizes.
-template <typename T, bool TA, bool TB, int MODE>
+template <typename T, bool TA, bool TB, int MODE, int SIDE>
 __global__ __launch_bounds__(256, 2) void k_product(Args g) {
-    using SA = Stage<T, TA>;
-    using SB = Stage<T, TB>;
-    __shared__ __attribute__((aligned(16))) char lds[2][SA::BYTES + SB::BYTES];
-    static_assert(4 * EPI_BYTES <= sizeof(lds), "the epilogue shares the operands' LDS");
-    const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b);
-    const float *bias = g.bias;
-    long long t;
-    int u;
-    map_tile(blockIdx.x, g.ti, g.tj, t, u);
-    long long i0 = 128 * t, i1 = g.I, r0 = 0, r1 = g.R;
-    const int j0 = 128 * u;
-    bool tail = false;
-    if (MODE == GROUP_ROWS) {
-        const Span s = find_group(g.counts, g.E, g.T, 128, t, -1);
-        if (s.e < 0 || (s.e == g.E && !g.zero_tail)) return;
-        i0 = s.start + 128 * s.tile;
-        i1 = s.end;
-        if (s.e == g.E) {
-            tail = true;
-            r1 = 0;
-        } else {
-            B += s.e * g.gstride;
-            if (bias) bias += (long long)s.e * g.J;
-        }
-    }
-    if (MODE == GROUP_RED) {
-        const Span s = find_group(g.counts, g.E, g.T, 1, 0, blockIdx.y);
-        r0 = s.start;
-        r1 = s.end;
-    }
-    if (g.splits > 1) {  // this slice of the reduction, whole steps
-        const long long steps = (r1 - r0 + SA::BK - 1) / SA::BK, per = (steps + g.splits - 1) / g.splits;
-        r0 = min(r1, r0 + blockIdx.z * per * SA::BK);
-        r1 = min(r1, r0 + per * SA::BK);
-    }
-
-    const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int wi = (wid >> 1) * 64, wj = (wid & 1) * 64;
-    f4 acc[4][4];
+    using SA = Stage<T, TA, SIDE>;
+    using SB = Stage<T, TB, SIDE>;
+    constexpr int Q = SIDE / 2, N = Q / 16;  // a wave's quarter, its MFMA tiles each way
+    constexpr int STEP = SA::BYTES + SB::BYTES;
+    __shared__ __attribute__((aligned(16))) char lds[2 * STEP];
+    static_assert(4 * epi_bytes(Q) <= (int)sizeof(lds), "the epilogue takes the operands' LDS");
+    const Work work = list_work<MODE>(g, SIDE);
+    if ((int)blockIdx.x >= work.n) return;
+    const Where w = locate<MODE>(g, work, blockIdx.x, SIDE, SIDE, SA::BK);
+    const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b) + w.boff;
+    const int wid = threadIdx.x >> 6, wi = (wid >> 1) * Q, wj = (wid & 1) * Q;
+    f4 acc[N][N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < N; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-    u4 va[4], vb[4];
-    const long long steps = (r1 - r0 + SA::BK - 1) / SA::BK;
+    u4 va[SA::N], vb[SB::N];
+    const long long steps = (w.r1 - w.r0 + SA::BK - 1) / SA::BK;
     if (steps > 0) {
-        SA::load(A, g.lda, i0, i1, r0, r1, va);
-        SB::load(B, g.ldb, j0, g.J, r0, r1, vb);
-        SA::write(lds[0], va);
-        SB::write(lds[0] + SA::BYTES, vb);
+        SA::load(A, g.lda, w.i0, w.i1, w.r0, w.r1, va);
+        SB::load(B, g.ldb, w.j0, g.J, w.r0, w.r1, vb);
+        SA::write(lds, va);
+        SB::write(lds + SA::BYTES, vb);
     }
     for (long long s = 0; s < steps; ++s) {
         __syncthreads();
         if (s + 1 < steps) {
-            SA::load(A, g.lda, i0, i1, r0 + (s + 1) * SA::BK, r1, va);
-            SB::load(B, g.ldb, j0, g.J, r0 + (s + 1) * SA::BK, r1, vb);
+            SA::load(A, g.lda, w.i0, w.i1, w.r0 + (s + 1) * SA::BK, w.r1, va);
+            SB::load(B, g.ldb, w.j0, g.J, w.r0 + (s + 1) * SA::BK, w.r1, vb);
         }
-        const char *la = lds[s & 1], *lb = la + SA::BYTES;
+        const char *la = lds + (s & 1) * STEP, *lb = la + SA::BYTES;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            u4 fa[4], fb[4];
+            u4 fa[N], fb[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = SA::frag(la, wi + 16 * i, h);
+            for (int i = 0; i < N; ++i) fa[i] = SA::frag(la, wi + 16 * i, h);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fb[j] = SB::frag(lb, wj + 16 * j, h);
+            for (int j = 0; j < N; ++j) fb[j] = SB::frag(lb, wj + 16 * j, h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
+                for (int j = 0; j < N; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
         }
         if (s + 1 < steps) {
-            SA::write(lds[(s + 1) & 1], va);
-            SB::write(lds[(s + 1) & 1] + SA::BYTES, vb);
+            SA::write(lds + ((s + 1) & 1) * STEP, va);
+            SB::write(lds + ((s + 1) & 1) * STEP + SA::BYTES, vb);
         }
     }
-
-    if (MODE == GROUP_RED) g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
     __syncthreads();  // the operands' buffers become the epilogue's
-    epilogue<T, MODE>(g, bias, tail, lds[0] + wid * EPI_BYTES, i0 + wi, i1, j0 + wj,
-                      [&](int i, int j) { return acc[i][j]; });
+    epilogue<T, Q, N>(
+        g, w, lds + wid * epi_bytes(Q), w.j0 + wj, [&](int p) { return w.i0 + wi + 16 * p; },
+        [&](int p, float *e) {
+            static_for<N>([&](auto i) {
+                if (p == i) {
+                    static_for<N>([&](auto j) { put_block<Q>(e, j, acc[i][j]); });
+                    asm volatile("; block %0" ::"n"(i.value));  // as in big_product
+                }
+            });
+        });
+}
+
+// ---- few rows -----------------------------------------------------------
+// x of at most a few rows (or groups of them) against a wide weight: what
+// counts is to stream the weight.  A workgroup takes 16 columns by 16 MT rows;
+// its waves share the reduction, each wave 128 bytes of every row at a time
+// (lane: row l & 15, two pieces at 32 (l >> 4) bytes), four such chunks in
+// flight, straight from memory into the MFMAs; the waves' sums meet in LDS.
+// Rows and columns beyond the end are clamped: their products are not stored.
+template <typename T, int MODE, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
+    constexpr int N = VEC<T>, KC = 8 * N, U = 4, ROWS = 16 * MT;
+    __shared__ __attribute__((aligned(16))) float red[WAVES][ROWS][16];
+    const Work work = list_work<MODE>(g, ROWS);
+    if ((int)blockIdx.x >= work.n) return;
+    const Where w = locate<MODE>(g, work, blockIdx.x, ROWS, 16, 1);
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, f = lane & 15, q = lane >> 4;
+    const T *B = reinterpret_cast<const T *>(g.b) + w.boff + min(w.j0 + f, g.J - 1) * g.ldb;
+    const T *A[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) A[m] = reinterpret_cast<const T *>(g.a) + min(w.i0 + 16 * m + f, w.i1 - 1) * g.lda;
+    f4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
+    const int K = (int)w.r1, whole = K / KC;
+    if (!w.tail) {
+        int c = wid;
+        for (; c + (U - 1) * WAVES < whole; c += U * WAVES) {
+            u4 b[U][2];
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+                    b[k][p] = reinterpret_cast<const Un16<T> *>(B + (c + k * WAVES) * KC + (2 * q + p) * N)->v;
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        acc[m] = Mma<T>::mul(
+                            b[k][p],
+                            reinterpret_cast<const Un16<T> *>(A[m] + (c + k * WAVES) * KC + (2 * q + p) * N)->v, acc[m]);
+        }
+        for (; c * KC < K; c += WAVES)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int k = c * KC + (2 * q + p) * N;
+                const u4 b = load_piece(B + k, k, K - k);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::mul(b, load_piece(A[m] + k, k, K - k), acc[m]);
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<f4 *>(&red[wid][16 * m + f][4 * q]) = acc[m];
+    __syncthreads();
+    for (int t = threadIdx.x; t < ROWS * 16 / N; t += 64 * WAVES) {
+        const int r = t / (16 / N), c = t % (16 / N) * N;
+        if (w.i0 + r >= w.i1 || w.j0 + c >= g.J) continue;
+        float v[N] = {};
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] += red[k][r][c + e];
+        float b[N] = {};
+        if (g.bias && !w.tail) load_row<float, N>(g.bias + w.biasoff + w.j0 + c, w.j0 + c, g.J - w.j0 - c, b);
+        store_outputs<T>(g, w, w.i0 + r, w.j0 + c, v, b, load_residual<T>(g, w.i0 + r, w.j0 + c));
+    }
 }
 
 // ---- the large 16-bit tile ----------------------------------------------
@@ -526,17 +697,16 @@ __device__ __forceinline__ void big_barrier() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
 }
-// a value that is the same in all lanes, in scalar registers
-__device__ __forceinline__ long long uniform(long long v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    return (long long)((uint64_t)hi << 32 | lo);
-}
 // 16 bytes a lane from base + off to 1 KiB of LDS at dst (wave-uniform)
 __device__ __forceinline__ void dma16(const void *src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+                 "v"(src)
+                 : "memory");
 }
 __device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                     __builtin_amdgcn_readfirstlane(dst)),
+                 "v"(off), "s"(uniform((long long)(uintptr_t)base))
                  : "memory");
 }
 
@@ -554,7 +724,7 @@ template <typename T, bool TR, bool ISB> struct BigOperand {
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
             const int row = TR ? 4 * (2 * wid + d) + (lane >> 4) : 8 * (2 * wid + d) + (lane >> 3);
-            const int pc = (TR ? lane & 15 : lane & 7) ^ Stage<T, TR>::swz(row);
+            const int pc = (TR ? lane & 15 : lane & 7) ^ Stage<T, TR, 128>::swz(row);
             r[d] = TR ? row : 8 * pc;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -577,53 +747,32 @@ template <typename T, bool TR, bool ISB> struct BigOperand {
     }
 };
 
+// Tile id of a product.  (Persistent workgroups, which had the next tile's
+// first K-tiles on their way during the epilogue, spilled around it and were
+// 5 to 45 % slower than a workgroup per tile.)
 template <typename T, bool TA, bool TB, int MODE>
-__global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const char *A = reinterpret_cast<const char *>(g.a), *B = reinterpret_cast<const char *>(g.b);
-    const float *bias = g.bias;
-    long long t;
-    int u;
-    map_tile(blockIdx.x, g.ti, g.tj, t, u);
-    long long i0 = BIG * t, i1 = g.I, r0 = 0, r1 = g.R;
-    const int j0 = BIG * u;
-    bool tail = false;
-    if (MODE == GROUP_ROWS) {
-        const Span s = find_group(g.counts, g.E, g.T, BIG, t, -1);
-        if (s.e < 0 || (s.e == g.E && !g.zero_tail)) return;
-        i0 = s.start + BIG * s.tile;
-        i1 = s.end;
-        if (s.e == g.E) {
-            tail = true;
-        } else {
-            B += s.e * g.gstride * 2;
-            if (bias) bias += (long long)s.e * g.J;
-        }
-    }
-    if (MODE == GROUP_RED) {
-        const Span s = find_group(g.counts, g.E, g.T, 1, 0, blockIdx.y);
-        r0 = s.start;
-        r1 = s.end;
-    }
-    if (g.splits > 1) {
-        const long long steps = (r1 - r0 + 63) / 64, per = (steps + g.splits - 1) / g.splits;
-        r0 = min(r1, r0 + blockIdx.z * per * 64);
-        r1 = min(r1, r0 + per * 64);
-    }
+__device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
+    const Work work = list_work<MODE>(g, BIG);
+    if (id >= work.n) return;
+    const Where w = locate<MODE>(g, work, id, BIG, BIG, 64);
+    using std::integral_constant;
+    constexpr integral_constant<int, 0> c0{};
+    constexpr integral_constant<int, 1> c1{};
+    constexpr integral_constant<int, 2> c2{};
+    constexpr integral_constant<int, 3> c3{};
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int grp = wid >> 2, wn = wid & 3, f = lane & 15, q = lane >> 4;
-
+    const int grp = wid >> 2, wn = wid & 3;
+    const uint32_t dst = (uint32_t)(uintptr_t)(lds_s4)lds + 2048u * wid;
     f4 acc[2][2][4][2];
 #pragma unroll
     for (int k = 0; k < 32; ++k) acc[k >> 4][(k >> 3) & 1][(k >> 1) & 3][k & 1] = f4{0.f, 0.f, 0.f, 0.f};
 
-    if (!tail) {
+    if (!w.tail) {
         BigOperand<T, TA, false> oa;
         BigOperand<T, TB, true> ob;
-        oa.init(A, g.lda, i0, i1, r0, wid, lane);
-        ob.init(B, g.ldb, j0, g.J, r0, wid, lane);
-        const long long len = uniform(r1 - r0), KT = max(4ll, (len + 127) / 128 * 2);
-        const uint32_t dst = (uint32_t)(uintptr_t)(lds_s4)lds + 2048u * wid;
+        oa.init(g.a, g.lda, w.i0, w.i1, w.r0, wid, lane);
+        ob.init(reinterpret_cast<const T *>(g.b) + w.boff, g.ldb, w.j0, g.J, w.r0, wid, lane);
+        const long long len = uniform(w.r1 - w.r0), KT = max(4ll, (len + 127) / 128 * 2);
 
         // half-tile Q (B0 A0 B1 A1) of K-tile tt into buffer PAR
         auto issue = [&](auto Q, auto Par, auto Part, long long tt) {
@@ -648,14 +797,14 @@ __global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) fa[s][i] = Stage<T, TA>::frag(p, 64 * grp + 16 * i, s);
+                for (int i = 0; i < 4; ++i) fa[s][i] = Stage<T, TA, 128>::frag(p, 64 * grp + 16 * i, s);
         };
         auto read_b = [&](u4 (&fb)[2][2], int h, int par) {
             const char *p = lds + par * BIG_BUF + (2 + h) * BIG_HALF;
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) fb[s][j] = Stage<T, TB>::frag(p, 32 * wn + 16 * j, s);
+                for (int j = 0; j < 2; ++j) fb[s][j] = Stage<T, TB, 128>::frag(p, 32 * wn + 16 * j, s);
         };
         auto mul = [&](f4 (&c)[4][2], const u4 (&fb)[2][2]) {
             big_barrier();
@@ -669,11 +818,6 @@ __global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
             __builtin_amdgcn_s_setprio(0);
             big_barrier();
         };
-        using std::integral_constant;
-        constexpr integral_constant<int, 0> c0{};
-        constexpr integral_constant<int, 1> c1{};
-        constexpr integral_constant<int, 2> c2{};
-        constexpr integral_constant<int, 3> c3{};
         // one K-tile in buffer PAR; END: 0 and 3 issue K-tile tt + 2 (3: which
         // may be partial), 1 and 2 are the last two
         auto tile = [&](auto End, auto Par, long long tt, u4 (&x)[2][2], u4 (&y)[2][2]) {
@@ -713,15 +857,25 @@ __global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
         tile(c3, c1, KT - 3, fy, fx);
         tile(c1, c0, KT - 2, fx, fy);
         tile(c2, c1, KT - 1, fy, fx);
-        if (grp == 0) big_barrier();  // every wave crosses as many
+        if (grp == 0) big_barrier();  // every wave crosses as many, and has read all of this tile
     }
+    epilogue<T, 64, 8>(
+        g, w, lds + wid * epi_bytes(64), w.j0 + 64 * wn,
+        [&](int p) { return w.i0 + 128 * (p >> 2) + 64 * grp + 16 * (p & 3); },
+        [&](int p, float *e) {
+            static_for<8>([&](auto k) {
+                if (p == k) {
+                    static_for<4>([&](auto j) { put_block<64>(e, j, acc[k >> 2][j >> 1][k & 3][j & 1]); });
+                    asm volatile("; block %0" ::"n"(k.value));  // the branches stay apart: merged, they would
+                }                                               // index the accumulators, in memory
+            });
+        });
+}
 
-    if (MODE == GROUP_RED) g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
-    __syncthreads();  // the operands' buffers become the epilogue's
-#pragma unroll
-    for (int hi = 0; hi < 2; ++hi)
-        epilogue<T, MODE>(g, bias, tail, lds + wid * EPI_BYTES, i0 + 128 * hi + 64 * grp, i1, j0 + 64 * wn,
-                          [&](int i, int j) { return acc[hi][j >> 1][i][j & 1]; });
+template <typename T, bool TA, bool TB, int MODE>
+__global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    big_product<T, TA, TB, MODE>(g, lds, blockIdx.x);
 }
 
 // The slices' partial sums, added in their order (no atomics: the same result
@@ -736,17 +890,19 @@ __global__ __launch_bounds__(256) void k_product_join(Args g) {
     const long long E = gridDim.y;
     float v[N] = {}, w[N];
     for (int s = 0; s < g.splits; ++s) {
-        load_row<float, N>(g.part + ((s * E + blockIdx.y) * g.I + row) * g.J + col, g.J - col, w);
+        load_row<float, N>(g.part + ((s * E + blockIdx.y) * g.I + row) * g.J + col, col, g.J - col, w);
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] += w[q];
     }
-    g.out = reinterpret_cast<T *>(g.out) + blockIdx.y * g.gstride;
-    finish<T>(g, g.bias, row, col, v);
+    float b[N] = {};
+    if (g.bias) load_row<float, N>(g.bias + col, col, g.J - col, b);
+    finish<T>(g, blockIdx.y * g.gstride, row, col, v, b, load_residual<T>(g, row, col));
 }
 
 // dz = dy act'(z) in T, and the column sums of dz before that rounding.  A
-// workgroup takes 128 columns (a lane 4, two rows at once per wave) of one
-// slice of one group's rows; sums go to part[group][slice][N].
+// workgroup takes one chunk of `rows` rows of a group by 32 pieces of 16 bytes;
+// its sums go to part[chunk][N], and k_bias_join adds a group's chunks.  Bound
+// by HBM: four rows of each thread are in flight at once.
 struct ActArgs {
     const void *dy, *z;
     long long ldy, ldz;
@@ -754,60 +910,100 @@ struct ActArgs {
     long long lddz;
     float *part;         // or null: dz only
     const int *counts;   // or null: one group of T rows
-    int E;
+    int E, rows;
     long long T;
     int N, act;
+    int zero_tail;       // write zeros to dz behind the last group
 };
 template <typename T>
 __global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
-    long long r0 = 0, r1 = g.T;
-    const int e = blockIdx.z;
+    constexpr int W = VEC<T>;
+    long long r0 = (long long)blockIdx.y * g.rows, r1 = min(g.T, r0 + g.rows);
+    bool tail = false;
     if (g.counts) {
-        const Span s = find_group(g.counts, g.E, g.T, 1, 0, e);
-        r0 = s.start;
-        r1 = s.end;
+        const Span s = find_group(g.counts, g.E, g.T, g.rows, blockIdx.y, -1);
+        tail = s.e == g.E;
+        if (s.e < 0 || (tail && !g.zero_tail)) return;
+        r0 = s.start + s.tile * g.rows;
+        r1 = min(s.end, r0 + g.rows);
     }
-    const long long per = (r1 - r0 + gridDim.y - 1) / gridDim.y;
-    r0 = min(r1, r0 + blockIdx.y * per);
-    r1 = min(r1, r0 + per);
-    const int c = blockIdx.x * 128 + (threadIdx.x & 31) * 4, n = g.N - c;
-    f4 sum{0.f, 0.f, 0.f, 0.f};
+    const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W, n = g.N - c;
+    const T *dy = reinterpret_cast<const T *>(g.dy) + c, *z = reinterpret_cast<const T *>(g.z) + c;
+    T *dz = reinterpret_cast<T *>(g.dz) + c;
+    float sum[W] = {};
     if (n > 0) {
-        for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-            f4 v{0.f, 0.f, 0.f, 0.f};
-            if (e < g.E) {
-                v = load4(reinterpret_cast<const T *>(g.dy) + r * g.ldy + c, n);
-                if (g.act != MDX_ACT_NONE) {
-                    const f4 z = load4(reinterpret_cast<const T *>(g.z) + r * g.ldz + c, n);
+        for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 32) {
+            float v[4][W], w[4][W];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = act_grad(v[q], z[q], g.act);
-                }
+            for (int k = 0; k < 4; ++k) {
+                const int m = r + 8 * k < r1 && !tail ? n : 0;
+                load_row<T, W>(dy + (m ? (r + 8 * k) * g.ldy : 0), c, m, v[k]);
+                if (g.act != MDX_ACT_NONE) load_row<T, W>(z + (m ? (r + 8 * k) * g.ldz : 0), c, m, w[k]);
             }
-            if (g.dz) store4(reinterpret_cast<T *>(g.dz) + r * g.lddz + c, v, n);
-            sum += v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (g.act != MDX_ACT_NONE && !tail)
+#pragma unroll
+                    for (int q = 0; q < W; ++q) v[k][q] = act_grad(v[k][q], w[k][q], g.act);
+                if (g.dz && r + 8 * k < r1) store_row<T, W>(dz + (r + 8 * k) * g.lddz, n, v[k]);
+#pragma unroll
+                for (int q = 0; q < W; ++q) sum[q] += v[k][q];
+            }
         }
     }
-    if (!g.part || e >= g.E) return;
-    __shared__ f4 sh[8][32];
-    sh[threadIdx.x >> 5][threadIdx.x & 31] = sum;
-    __syncthreads();
-    if (threadIdx.x < 32 && n > 0) {
+    if (!g.part || tail) return;
+    __shared__ float sh[8][32 * W];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) sum += sh[w][threadIdx.x];
-        store4(g.part + ((long long)e * gridDim.y + blockIdx.y) * g.N + c, sum, n);
+    for (int q = 0; q < W; ++q) sh[threadIdx.x >> 5][(threadIdx.x & 31) * W + q] = sum[q];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 32 * W; k += 256) {
+        const int col = blockIdx.x * 32 * W + k;
+        float v = sh[0][k];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) v += sh[w][k];
+        if (col < g.N) g.part[(long long)blockIdx.y * g.N + col] = v;
     }
 }
-// db[e][n] = the slices' sums in their order
-__global__ __launch_bounds__(256) void k_bias_join(const float *part, int slices, int N, float *db) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+// db[e][n] = the sums of group e's chunks, always added in the same order.  A
+// workgroup has 16 columns and 16 threads to each, so that a hundred chunks are
+// a few loads in flight per thread and no chain of waits.
+__global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) {
+    __shared__ float sh[4][16];
+    const int l = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + l;
+    long long first = 0, n = (g.T + g.rows - 1) / g.rows;
+    if (g.counts) {
+        const Span s = find_group(g.counts, g.E, g.T, g.rows, 0, blockIdx.y);
+        first = s.tile0;
+        n = (s.end - s.start + g.rows - 1) / g.rows;
+    }
     float v = 0.f;
-    for (int s = 0; s < slices; ++s) v += part[((long long)blockIdx.y * slices + s) * N + n];
-    db[(long long)blockIdx.y * N + n] = v;
+    if (col < g.N) {
+        const float *p = g.part + first * g.N + col;
+        for (long long k = w; k < n; k += 8 * 16) {
+            float t[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) t[q] = k + 16 * q < n ? p[(k + 16 * q) * g.N] : 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += t[q];
+        }
+    }
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][l] = v;
+    __syncthreads();
+    if (threadIdx.x < 16 && col < g.N) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v += sh[k][l];
+        db[(long long)blockIdx.y * g.N + col] = v;
+    }
 }
 
 // ---- host ---------------------------------------------------------------
 static long long ceil128(long long n) { return (n + 127) / 128; }
+
+// rows of a forward call that k_product_few takes (grouped: on average)
+constexpr int FEW = 64;
 
 // slices of the reduction: enough workgroups for two on each of the 256 CUs,
 // each of at least 4 steps of 128 bytes
@@ -817,14 +1013,20 @@ static int choose_splits(long long tiles, long long R, int es) {
     return (int)std::max<long long>(1, std::min<long long>(s, 16));
 }
 static int fwd_splits(long long M, int N, int K, int dtype) {
+    if (M <= FEW) return 1;
     return choose_splits(ceil128(M) * ceil128(N), K, dtype == 0 ? 4 : 2);
 }
 static int dw_splits(int E, long long T, int N, int K, int dtype) {
     return choose_splits((long long)E * ceil128(N) * ceil128(K), T / std::max(E, 1), dtype == 0 ? 4 : 2);
 }
-static int act_slices(int E, long long T, int N) {
-    const long long want = std::max<long long>(1, 1024 / (ceil128(N) * E));
-    return (int)std::max<long long>(1, std::min<long long>(want, (T / std::max(E, 1) + 31) / 32));
+// rows of a chunk of k_act_backward: about eight workgroups for each CU
+static int act_rows(long long T, int N, int dtype) {
+    const long long cols = ceil_div(N, dtype == 0 ? 128 : 256);
+    return (int)std::max<long long>(32, ceil_div(T * cols / 2048, 32) * 32);
+}
+// chunks of T rows in E groups (0: dense), and the rows behind them
+static long long act_chunks(int E, long long T, int rows) {
+    return std::max<long long>(1, ceil_div(T, rows)) + (E ? E + 1 : 0);
 }
 
 // the large tile: both operands in whole aligned pieces of 16 bytes, and
@@ -839,32 +1041,63 @@ template <typename T, bool TA, bool TB> static bool use_big(const Args &g, int m
     const long long groups = mode == GROUP_RED ? g.E : 1;
     return ceil_div(g.I, BIG) * ceil_div(g.J, BIG) * groups * g.splits >= 128;
 }
-
-template <typename T, bool TA, bool TB, int MODE> static int launch_product(Args g, hipStream_t s) {
-    const bool big = use_big<T, TA, TB>(g, MODE);
-    const int side = big ? BIG : 128, threads = big ? 512 : 256;
-    const long long bound = MODE == GROUP_ROWS ? g.E + 1 : 0;  // one partial tile more for each group
-    const long long ti = ceil_div(g.I, side) + bound, tj = ceil_div(g.J, side);
-    MDX_REQUIRE(ti * tj * threads < (1ll << 32), "mdx_linear: too many output tiles");
+// grid of tiles bi x bj; grouped rows: one partial tile more for each group,
+// and for the rows behind them; at most `most` workgroups
+constexpr int CUS = 256;  // of an MI355X; a multiple of its XCDs
+static int set_grid(Args &g, int mode, int bi, int bj, int threads, int most, dim3 &grid) {
+    const long long ti = ceil_div(g.I, bi) + (mode == GROUP_ROWS ? g.E + 1 : 0), tj = ceil_div(g.J, bj);
+    const long long n = ti * tj * (mode == GROUP_RED ? g.E : 1) * g.splits;
+    MDX_REQUIRE(n < (1ll << 31) && std::min<long long>(n, most) * threads < (1ll << 32),
+                "mdx_linear: too many output tiles");
     g.ti = (int)ti;
     g.tj = (int)tj;
-    const dim3 grid((unsigned)(ti * tj), MODE == GROUP_RED ? g.E : 1, g.splits);
+    grid = dim3((unsigned)std::min<long long>(n, most));
+    return MDX_OK;
+}
+template <typename T, bool TA, bool TB, int MODE> static int launch_product(Args g, hipStream_t s) {
+    dim3 grid;
+    int rc = MDX_OK;
+    bool done = false;
     if constexpr (sizeof(T) == 2) {
-        if (big) {
+        if (use_big<T, TA, TB>(g, MODE)) {
             static const hipError_t attr = hipFuncSetAttribute(
                 reinterpret_cast<const void *>(k_product_big<T, TA, TB, MODE>),
                 hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
             MDX_HIP(attr);
+            if ((rc = set_grid(g, MODE, BIG, BIG, 512, INT32_MAX, grid))) return rc;
             hipLaunchKernelGGL((k_product_big<T, TA, TB, MODE>), grid, dim3(512), BIG_LDS, s, g);
+            done = true;
         }
     }
-    if (!big) hipLaunchKernelGGL((k_product<T, TA, TB, MODE>), grid, dim3(256), 0, s, g);
+    const long long groups = MODE == GROUP_RED ? g.E : 1;
+    if (!done && ceil128(g.I) * ceil128(g.J) * groups * g.splits >= 256) {
+        if ((rc = set_grid(g, MODE, 128, 128, 256, INT32_MAX, grid))) return rc;
+        hipLaunchKernelGGL((k_product<T, TA, TB, MODE, 128>), grid, dim3(256), 0, s, g);
+    } else if (!done) {
+        if ((rc = set_grid(g, MODE, 64, 64, 256, INT32_MAX, grid))) return rc;
+        hipLaunchKernelGGL((k_product<T, TA, TB, MODE, 64>), grid, dim3(256), 0, s, g);
+    }
     MDX_CHECK_LAUNCH("mdx_linear");
     if (g.splits > 1) {
         const dim3 jg((unsigned)ceil_div(g.I * ceil_div(g.J, VEC<T>), 256), MODE == GROUP_RED ? g.E : 1);
         hipLaunchKernelGGL(k_product_join<T>, jg, dim3(256), 0, s, g);
         MDX_CHECK_LAUNCH("mdx_linear");
     }
+    return MDX_OK;
+}
+
+// few rows to a group: 16, 32 or 64 of them in a tile, 4, 8 or 16 waves to the reduction
+template <typename T, int MODE, int MT> static int launch_few(Args g, hipStream_t s) {
+    const long long chunks = ceil_div(g.R * (long long)sizeof(T), 128);
+    const int waves = chunks >= 128 ? 16 : chunks >= 32 ? 8 : 4;
+    dim3 grid;
+    if (int rc = set_grid(g, MODE, 16 * MT, 16, 64 * waves, INT32_MAX, grid)) return rc;
+    switch (waves) {
+        case 16: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 16>), grid, dim3(1024), 0, s, g); break;
+        case 8: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 8>), grid, dim3(512), 0, s, g); break;
+        default: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 4>), grid, dim3(256), 0, s, g);
+    }
+    MDX_CHECK_LAUNCH("mdx_linear");
     return MDX_OK;
 }
 
@@ -882,9 +1115,15 @@ static int check_shape(const char *fn, const Shape &p) {
 }
 static bool bad_ld(const void *p, long long ld, long long width) { return p && ld < width; }
 
-template <typename T> static int forward(const Shape &p, Args g, hipStream_t s) {
-    if (p.E) return launch_product<T, false, false, GROUP_ROWS>(g, s);
-    return launch_product<T, false, false, DENSE>(g, s);
+template <typename T, int MODE> static int forward_mode(const Shape &p, const Args &g, hipStream_t s) {
+    const long long rows = ceil_div(p.T, std::max(p.E, 1));
+    if (rows <= 16) return launch_few<T, MODE, 1>(g, s);
+    if (rows <= 32) return launch_few<T, MODE, 2>(g, s);
+    if (rows <= FEW) return launch_few<T, MODE, 4>(g, s);
+    return launch_product<T, false, false, MODE>(g, s);
+}
+template <typename T> static int forward(const Shape &p, const Args &g, hipStream_t s) {
+    return p.E ? forward_mode<T, GROUP_ROWS>(p, g, s) : forward_mode<T, DENSE>(p, g, s);
 }
 
 struct Back {
@@ -900,7 +1139,7 @@ struct Back {
 // workspace: dz | sums of db | partial dW, each 256-B aligned
 struct BackPlan {
     bool sums, dz;  // the elementwise pass: for its sums, for dz in the workspace
-    int slices, splits;
+    int rows, splits;  // of a chunk of the elementwise pass; slices of dw's reduction
     long long dz_bytes, part_bytes, dw_bytes;
 };
 static long long up256(long long n) { return (n + 255) / 256 * 256; }
@@ -909,10 +1148,10 @@ static BackPlan plan_backward(const Shape &p, bool need_x, bool need_w, bool nee
     const int E = std::max(p.E, 1), es = p.dtype == 0 ? 4 : 2;
     q.sums = need_b;
     q.dz = p.act != MDX_ACT_NONE && (need_x || need_w) && !need_r;
-    q.slices = act_slices(E, p.T, p.N);
+    q.rows = act_rows(p.T, p.N, p.dtype);
     q.splits = need_w ? dw_splits(E, p.T, p.N, p.K, p.dtype) : 1;
     q.dz_bytes = q.dz ? up256(p.T * p.N * es) : 0;
-    q.part_bytes = need_b ? up256((long long)E * q.slices * p.N * 4) : 0;
+    q.part_bytes = need_b ? up256(act_chunks(p.E, p.T, q.rows) * p.N * 4) : 0;
     q.dw_bytes = q.splits > 1 ? up256((long long)q.splits * E * p.N * p.K * 4) : 0;
     return q;
 }
@@ -931,14 +1170,15 @@ template <typename T> static int backward(const Shape &p, const Back &b, hipStre
         a.lddz = b.dres ? b.lddr : p.N;
         a.part = b.db ? part : nullptr;
         a.counts = b.counts;
-        a.E = E; a.T = p.T; a.N = p.N; a.act = p.act;
-        const bool tail = p.E && b.dres && b.zero_tail;
-        const dim3 grid((unsigned)ceil128(p.N), q.slices, E + tail);
+        a.E = p.E; a.T = p.T; a.N = p.N; a.act = p.act;
+        a.rows = q.rows;
+        a.zero_tail = b.dres && b.zero_tail;
+        const long long chunks = act_chunks(p.E, p.T, q.rows);
+        const dim3 grid((unsigned)ceil_div(p.N, 32 * VEC<T>), (unsigned)chunks);
         hipLaunchKernelGGL(k_act_backward<T>, grid, dim3(256), 0, s, a);
         MDX_CHECK_LAUNCH("mdx_linear_backward");
         if (b.db) {
-            hipLaunchKernelGGL(k_bias_join, dim3((unsigned)ceil_div(p.N, 256), E), dim3(256), 0, s, part, q.slices,
-                               p.N, b.db);
+            hipLaunchKernelGGL(k_bias_join, dim3((unsigned)ceil_div(p.N, 16), E), dim3(256), 0, s, a, b.db);
             MDX_CHECK_LAUNCH("mdx_linear_backward");
         }
         if (a.dz && p.act != MDX_ACT_NONE) {
