@@ -13,6 +13,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace mdx {
@@ -136,10 +137,35 @@ __device__ __forceinline__ float act_slope(float z, int act) {
         default: return 1.f;
     }
 }
+// a whole piece: the activation is chosen once, not for each element
+template <int ACT, int N> __device__ __forceinline__ void apply(float (&v)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = act_value(v[q], ACT);
+}
+template <int N> __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
+    switch (act) {
+        case MDX_ACT_RELU: return apply<MDX_ACT_RELU>(v);
+        case MDX_ACT_GELU: return apply<MDX_ACT_GELU>(v);
+        case MDX_ACT_GELU_TANH: return apply<MDX_ACT_GELU_TANH>(v);
+        case MDX_ACT_SILU: return apply<MDX_ACT_SILU>(v);
+    }
+}
 // dy act'(z); ReLU selects, so that an infinite gradient of a closed unit is dropped
 __device__ __forceinline__ float act_grad(float dy, float z, int act) {
     if (act == MDX_ACT_RELU) return z > 0.f ? dy : 0.f;
     return dy * act_slope(z, act);
+}
+template <int ACT, int N> __device__ __forceinline__ void apply_grad(float (&v)[N], const float (&z)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = act_grad(v[q], z[q], ACT);
+}
+template <int N> __device__ __forceinline__ void apply_act_grad(float (&v)[N], const float (&z)[N], int act) {
+    switch (act) {
+        case MDX_ACT_RELU: return apply_grad<MDX_ACT_RELU>(v, z);
+        case MDX_ACT_GELU: return apply_grad<MDX_ACT_GELU>(v, z);
+        case MDX_ACT_GELU_TANH: return apply_grad<MDX_ACT_GELU_TANH>(v, z);
+        case MDX_ACT_SILU: return apply_grad<MDX_ACT_SILU>(v, z);
+    }
 }
 
 // ---- one product --------------------------------------------------------
@@ -342,9 +368,7 @@ __device__ __forceinline__ void finish(const Args &g, long long ooff, long long 
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] += (float)r.e[q];
     if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i * g.ldp + j, n, v);
-    if (g.act != MDX_ACT_NONE)
-#pragma unroll
-        for (int q = 0; q < N; ++q) v[q] = act_value(v[q], g.act);
+    apply_act(v, g.act);
     store_row<T, N>(reinterpret_cast<T *>(g.out) + ooff + i * g.ldo + j, n, v);
 }
 template <typename T> __device__ __forceinline__ u4 load_residual(const Args &g, long long i, int j) {
@@ -425,24 +449,30 @@ __device__ __forceinline__ void epilogue(const Args &g, const Where &w, char *ld
     }
 }
 
-template <typename T> struct Mma;
-template <> struct Mma<__bf16> {
-    static __device__ __forceinline__ f4 mul(u4 x, u4 y, f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+// 16 x 16 sums over a fragment of 16 bytes of each operand, in STEPS instructions
+template <typename T> struct Mma {
+    static constexpr int STEPS = 1;
+    static __device__ __forceinline__ f4 mul_step(u4 x, u4 y, f4 c, int) {
+        if constexpr (std::is_same<T, __bf16>::value)
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0,
+                                                           0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0,
+                                                          0);
     }
-};
-template <> struct Mma<_Float16> {
-    static __device__ __forceinline__ f4 mul(u4 x, u4 y, f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
-    }
+    static __device__ __forceinline__ f4 mul(u4 x, u4 y, f4 c) { return mul_step(x, y, c, 0); }
 };
 template <> struct Mma<float> {
-    // element e of lane (row, q) is r = 4 q + e in both operands: any order of
+    // element k of lane (row, q) is r = 4 q + k in both operands: any order of
     // the products gives the same sum
+    static constexpr int STEPS = 4;
+    static __device__ __forceinline__ f4 mul_step(u4 x, u4 y, f4 c, int k) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, x)[k], __builtin_bit_cast(f4, y)[k], c, 0, 0,
+                                                    0);
+    }
     static __device__ __forceinline__ f4 mul(u4 x, u4 y, f4 c) {
-        const f4 a = __builtin_bit_cast(f4, x), b = __builtin_bit_cast(f4, y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        for (int k = 0; k < 4; ++k) c = mul_step(x, y, c, k);
         return c;
     }
 };
@@ -511,60 +541,166 @@ template <typename T, bool TR, int SIDE> struct Stage {
     }
 };
 
+// ---- LDS-DMA --------------------------------------------------------------
+__device__ __attribute__((aligned(64))) uint4 zero_piece[4];  // what lies beyond the reduction's end
+
+// Waits and barriers that no memory access is moved across.  The DMA is
+// inline asm, so that the compiler, which would wait for all of it before any
+// LDS read, leaves the count of outstanding ones to these waits.
+template <int VM> __device__ __forceinline__ void dma_wait() {  // vmcnt VM, lgkmcnt 0, any expcnt
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | 0x70);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void dma_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+// 16 bytes a lane from base + off to 1 KiB of LDS at dst (wave-uniform)
+__device__ __forceinline__ void dma16(const void *src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
+                 "v"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                     __builtin_amdgcn_readfirstlane(dst)),
+                 "v"(off), "s"(uniform((long long)(uintptr_t)base))
+                 : "memory");
+}
+
+// ---- the small tiles ------------------------------------------------------
 // Tile SIDE x SIDE (128 or 64) per workgroup of 4 waves, each a quarter of 16 x
-// 16 MFMA tiles; the reduction in steps of 128 bytes through two LDS buffers,
-// the next step's global loads in flight in registers meanwhile.  B is the
-// MFMA's first operand, so a lane ends with 4 neighbouring columns of one row.
-// Any alignment, any sizes.
-template <typename T, bool TA, bool TB, int MODE, int SIDE>
-__global__ __launch_bounds__(256, 2) void k_product(Args g) {
+// 16 MFMA tiles, the reduction in steps of 128 bytes.  B is the MFMA's first
+// operand, so a lane ends with 4 neighbouring columns of one row.
+//
+// DMA: both operands in aligned pieces of 16 bytes, brought to LDS directly,
+// BUFS - 1 steps ahead, so that a lone workgroup on a CU does not wait out the
+// memory's latency at each step; one barrier a step, behind which step s has
+// landed everywhere and step s - 1 has been read, so that its buffer is free.
+// Otherwise: any alignment and sizes, through registers, one step ahead.
+template <typename T, int SIDE, bool DMA> constexpr int BUFS = !DMA || (sizeof(T) == 4 && SIDE == 128) ? 2 : 4;
+
+// a lane's part in staging one operand by DMA: instruction d of wave w brings
+// 1 KiB, rows (w SIDE / 32 + d) 64 / PPR ..
+template <typename T, bool TR, int SIDE> struct SmallOperand {
+    using S = Stage<T, TR, SIDE>;
+    const char *base;  // first piece of step 0
+    long long step;    // bytes between steps
+    uint32_t off[S::N];
+    int r[S::N];       // reduction index of the piece in its step
+    __device__ __forceinline__ void init(const T *p, long long ld, long long i0, long long I, long long r0, int wid) {
+        constexpr int ES = sizeof(T);
+        const int lane = threadIdx.x & 63;
+        base = reinterpret_cast<const char *>(
+            uniform((long long)(reinterpret_cast<uintptr_t>(p) + (TR ? r0 * ld + i0 : i0 * ld + r0) * ES)));
+        step = TR ? S::BK * ld * ES : 128;
+#pragma unroll
+        for (int d = 0; d < S::N; ++d) {
+            const int row = (wid * S::N + d) * (64 / S::PPR) + lane / S::PPR, pc = (lane % S::PPR) ^ S::swz(row);
+            const long long i = min(i0 + (TR ? pc * VEC<T> : row), TR ? I - VEC<T> : I - 1);
+            r[d] = TR ? row : pc * VEC<T>;
+            off[d] = (uint32_t)(TR ? (row * ld + i - i0) * ES : (i - i0) * ld * ES + 16 * pc);
+        }
+    }
+    __device__ __forceinline__ void issue(long long s, long long left, uint32_t dst) const {
+        if (left >= S::BK) {
+#pragma unroll
+            for (int d = 0; d < S::N; ++d) dma16s(base + s * step, off[d], dst + 1024 * d);
+        } else {
+#pragma unroll
+            for (int d = 0; d < S::N; ++d)
+                dma16(r[d] < left ? base + s * step + off[d] : reinterpret_cast<const char *>(zero_piece),
+                      dst + 1024 * d);
+        }
+    }
+};
+
+template <typename T, bool TA, bool TB, int MODE, int SIDE, bool DMA>
+__device__ __forceinline__ void small_product(const Args &g, char *lds, int id) {
     using SA = Stage<T, TA, SIDE>;
     using SB = Stage<T, TB, SIDE>;
     constexpr int Q = SIDE / 2, N = Q / 16;  // a wave's quarter, its MFMA tiles each way
-    constexpr int STEP = SA::BYTES + SB::BYTES;
-    __shared__ __attribute__((aligned(16))) char lds[2 * STEP];
-    static_assert(4 * epi_bytes(Q) <= (int)sizeof(lds), "the epilogue takes the operands' LDS");
+    constexpr int STEP = SA::BYTES + SB::BYTES, NB = BUFS<T, SIDE, DMA>;
+    static_assert(4 * epi_bytes(Q) <= 2 * STEP, "the epilogue takes the operands' LDS");
     const Work work = list_work<MODE>(g, SIDE);
-    if ((int)blockIdx.x >= work.n) return;
-    const Where w = locate<MODE>(g, work, blockIdx.x, SIDE, SIDE, SA::BK);
+    if (id >= work.n) return;
+    const Where w = locate<MODE>(g, work, id, SIDE, SIDE, SA::BK);
     const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b) + w.boff;
-    const int wid = threadIdx.x >> 6, wi = (wid >> 1) * Q, wj = (wid & 1) * Q;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = (wid >> 1) * Q, wj = (wid & 1) * Q;
     f4 acc[N][N];
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-
-    u4 va[SA::N], vb[SB::N];
-    const long long steps = (w.r1 - w.r0 + SA::BK - 1) / SA::BK;
-    if (steps > 0) {
-        SA::load(A, g.lda, w.i0, w.i1, w.r0, w.r1, va);
-        SB::load(B, g.ldb, w.j0, g.J, w.r0, w.r1, vb);
-        SA::write(lds, va);
-        SB::write(lds + SA::BYTES, vb);
-    }
-    for (long long s = 0; s < steps; ++s) {
-        __syncthreads();
-        if (s + 1 < steps) {
-            SA::load(A, g.lda, w.i0, w.i1, w.r0 + (s + 1) * SA::BK, w.r1, va);
-            SB::load(B, g.ldb, w.j0, g.J, w.r0 + (s + 1) * SA::BK, w.r1, vb);
-        }
-        const char *la = lds + (s & 1) * STEP, *lb = la + SA::BYTES;
+    auto read = [&](u4 (&fa)[2][N], u4 (&fb)[2][N], const char *la) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            u4 fa[N], fb[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) fa[i] = SA::frag(la, wi + 16 * i, h);
+            for (int i = 0; i < N; ++i) fa[h][i] = SA::frag(la, wi + 16 * i, h);
 #pragma unroll
-            for (int j = 0; j < N; ++j) fb[j] = SB::frag(lb, wj + 16 * j, h);
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[i][j] = Mma<T>::mul(fb[j], fa[i], acc[i][j]);
+            for (int j = 0; j < N; ++j) fb[h][j] = SB::frag(la + SA::BYTES, wj + 16 * j, h);
         }
-        if (s + 1 < steps) {
-            SA::write(lds + ((s + 1) & 1) * STEP, va);
-            SB::write(lds + ((s + 1) & 1) * STEP + SA::BYTES, vb);
+    };
+    auto multiply = [&](const u4 (&fa)[2][N], const u4 (&fb)[2][N]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < Mma<T>::STEPS; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) acc[i][j] = Mma<T>::mul_step(fb[h][j], fa[h][i], acc[i][j], k);
+    };
+    const long long len = uniform(w.r1 - w.r0), steps = (len + SA::BK - 1) / SA::BK;
+    if constexpr (DMA) {
+        SmallOperand<T, TA, SIDE> oa;
+        SmallOperand<T, TB, SIDE> ob;
+        if (steps > 0) {
+            oa.init(A, g.lda, w.i0, w.i1, w.r0, wid);
+            ob.init(B, g.ldb, w.j0, g.J, w.r0, wid);
+            const uint32_t dst = (uint32_t)(uintptr_t)(lds_s4)lds + 1024u * SA::N * wid;
+            auto issue = [&](long long s) {
+                const uint32_t d = dst + (uint32_t)(s % NB) * STEP;
+                oa.issue(s, len - s * SA::BK, d);
+                ob.issue(s, len - s * SA::BK, d + SA::BYTES);
+            };
+#pragma unroll
+            for (int s = 0; s < NB - 1; ++s) issue(s);
+            for (long long s = 0; s < steps; ++s) {
+                u4 fa[2][N], fb[2][N];
+                dma_wait<(NB - 2) * 2 * SA::N>();
+                dma_barrier();
+                read(fa, fb, lds + (s % NB) * STEP);
+                issue(s + NB - 1);  // beyond the end: zeros, so that the count stays the same
+                multiply(fa, fb);
+            }
+            dma_wait<0>();  // nothing may land in the epilogue's LDS
+        }
+    } else {
+        u4 va[SA::N], vb[SB::N];
+        if (steps > 0) {
+            SA::load(A, g.lda, w.i0, w.i1, w.r0, w.r1, va);
+            SB::load(B, g.ldb, w.j0, g.J, w.r0, w.r1, vb);
+            SA::write(lds, va);
+            SB::write(lds + SA::BYTES, vb);
+        }
+        for (long long s = 0; s < steps; ++s) {
+            __syncthreads();
+            if (s + 1 < steps) {
+                SA::load(A, g.lda, w.i0, w.i1, w.r0 + (s + 1) * SA::BK, w.r1, va);
+                SB::load(B, g.ldb, w.j0, g.J, w.r0 + (s + 1) * SA::BK, w.r1, vb);
+            }
+            u4 fa[2][N], fb[2][N];
+            read(fa, fb, lds + (s & 1) * STEP);
+            multiply(fa, fb);
+            if (s + 1 < steps) {
+                SA::write(lds + ((s + 1) & 1) * STEP, va);
+                SB::write(lds + ((s + 1) & 1) * STEP + SA::BYTES, vb);
+            }
         }
     }
     __syncthreads();  // the operands' buffers become the epilogue's
@@ -574,8 +710,8 @@ __global__ __launch_bounds__(256, 2) void k_product(Args g) {
             static_for<N>([&](auto i) {
                 if (p == i) {
                     static_for<N>([&](auto j) { put_block<Q>(e, j, acc[i][j]); });
-                    asm volatile("; block %0" ::"n"(i.value));  // as in big_product
-                }
+                    asm volatile("; block %0" ::"n"(i.value));  // the branches stay apart: merged, they would
+                }                                               // index the accumulators, in memory
             });
         });
 }
@@ -678,37 +814,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
 // outputs that are not stored); beyond the reduction's end both operands read
 // zeros, and the K-tiles are rounded up to an even number of at least 4; only
 // the first two and the last two can be partial.
-__device__ __attribute__((aligned(64))) uint4 zero_piece[4];
-
 constexpr int BIG = 256, BIG_BUF = 65536, BIG_LDS = 2 * BIG_BUF, BIG_HALF = 16384;
-
-// Waits and barriers that no memory access is moved across.  The DMA is
-// inline asm, so that the compiler, which would wait for all of it before any
-// LDS read, leaves the count of outstanding ones to these waits.
-template <int VM> __device__ __forceinline__ void big_wait() {  // vmcnt VM, lgkmcnt 0, any expcnt
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | 0x70);
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void big_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-}
-// 16 bytes a lane from base + off to 1 KiB of LDS at dst (wave-uniform)
-__device__ __forceinline__ void dma16(const void *src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
-                 "v"(src)
-                 : "memory");
-}
-__device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
-                     __builtin_amdgcn_readfirstlane(dst)),
-                 "v"(off), "s"(uniform((long long)(uintptr_t)base))
-                 : "memory");
-}
 
 // a lane's part in staging and reading one operand
 template <typename T, bool TR, bool ISB> struct BigOperand {
@@ -807,7 +913,7 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
                 for (int j = 0; j < 2; ++j) fb[s][j] = Stage<T, TB, 128>::frag(p, 32 * wn + 16 * j, s);
         };
         auto mul = [&](f4 (&c)[4][2], const u4 (&fb)[2][2]) {
-            big_barrier();
+            dma_barrier();
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -816,7 +922,7 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) c[i][j] = Mma<T>::mul(fb[s][j], fa[s][i], c[i][j]);
             __builtin_amdgcn_s_setprio(0);
-            big_barrier();
+            dma_barrier();
         };
         // one K-tile in buffer PAR; END: 0 and 3 issue K-tile tt + 2 (3: which
         // may be partial), 1 and 2 are the last two
@@ -826,29 +932,29 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
             constexpr integral_constant<int, END == 3> part{};
             read_a(0, PAR);
             if constexpr (MORE) issue(c0, Par, part, tt + 2);
-            big_wait<MORE ? 12 : END == 1 ? 10 : 2>();
+            dma_wait<MORE ? 12 : END == 1 ? 10 : 2>();
             mul(acc[0][0], x);
             read_b(y, 1, PAR);
             if constexpr (MORE) issue(c1, Par, part, tt + 2);
-            big_wait<MORE ? 12 : END == 1 ? 8 : 0>();
+            dma_wait<MORE ? 12 : END == 1 ? 8 : 0>();
             mul(acc[0][1], y);
             read_a(1, PAR);
             if constexpr (MORE) issue(c2, Par, part, tt + 2);
-            big_wait<MORE ? 12 : END == 1 ? 6 : 0>();
+            dma_wait<MORE ? 12 : END == 1 ? 6 : 0>();
             mul(acc[1][1], y);
             if constexpr (END != 2) read_b(y, 0, 1 - PAR);
             if constexpr (MORE) issue(c3, Par, part, tt + 2);
-            big_wait<MORE ? 12 : END == 1 ? 4 : 0>();
+            dma_wait<MORE ? 12 : END == 1 ? 4 : 0>();
             mul(acc[1][0], x);
         };
         issue(c0, c0, c1, 0); issue(c1, c0, c1, 0); issue(c2, c0, c1, 0); issue(c3, c0, c1, 0);
         issue(c0, c1, c1, 1); issue(c1, c1, c1, 1); issue(c2, c1, c1, 1); issue(c3, c1, c1, 1);
-        big_wait<12>();
-        big_barrier();
+        dma_wait<12>();
+        dma_barrier();
         read_b(fx, 0, 0);
-        big_wait<12>();
-        big_barrier();
-        if (grp == 1) big_barrier();  // one behind
+        dma_wait<12>();
+        dma_barrier();
+        if (grp == 1) dma_barrier();  // one behind
         for (long long tt = 0; tt < KT - 4; tt += 2) {
             tile(c0, c0, tt, fx, fy);
             tile(c0, c1, tt + 1, fy, fx);
@@ -857,7 +963,7 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
         tile(c3, c1, KT - 3, fy, fx);
         tile(c1, c0, KT - 2, fx, fy);
         tile(c2, c1, KT - 1, fy, fx);
-        if (grp == 0) big_barrier();  // every wave crosses as many, and has read all of this tile
+        if (grp == 0) dma_barrier();  // every wave crosses as many, and has read all of this tile
     }
     epilogue<T, 64, 8>(
         g, w, lds + wid * epi_bytes(64), w.j0 + 64 * wn,
@@ -866,16 +972,45 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
             static_for<8>([&](auto k) {
                 if (p == k) {
                     static_for<4>([&](auto j) { put_block<64>(e, j, acc[k >> 2][j >> 1][k & 3][j & 1]); });
-                    asm volatile("; block %0" ::"n"(k.value));  // the branches stay apart: merged, they would
-                }                                               // index the accumulators, in memory
+                    asm volatile("; block %0" ::"n"(k.value));  // as in small_product
+                }
             });
         });
 }
 
-template <typename T, bool TA, bool TB, int MODE>
-__global__ __launch_bounds__(512, 2) void k_product_big(Args g) {
+// ---- kernels ----------------------------------------------------------------
+enum Kind { LARGE, DMA128, DMA64, REG128, REG64 };
+constexpr int tile_side(int kind) { return kind == LARGE ? BIG : kind == DMA128 || kind == REG128 ? 128 : 64; }
+constexpr int tile_threads(int kind) { return kind == LARGE ? 512 : 256; }
+template <typename T> constexpr int tile_lds(int kind) {
+    return kind == LARGE    ? BIG_LDS
+           : kind == DMA128 ? BUFS<T, 128, true> * 32768
+           : kind == DMA64  ? BUFS<T, 64, true> * 16384
+           : kind == REG128 ? 65536
+                            : 32768;
+}
+template <typename T, bool TA, bool TB, int MODE, int KIND>
+__device__ __forceinline__ void run_tile(const Args &g, char *lds, int id) {
+    if constexpr (KIND == LARGE)
+        big_product<T, TA, TB, MODE>(g, lds, id);
+    else
+        small_product<T, TA, TB, MODE, tile_side(KIND), KIND == DMA128 || KIND == DMA64>(g, lds, id);
+}
+template <typename T, int MODE, int KIND>
+__global__ __launch_bounds__(tile_threads(KIND), 2) void k_forward(Args g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    big_product<T, TA, TB, MODE>(g, lds, blockIdx.x);
+    run_tile<T, false, false, MODE, KIND>(g, lds, blockIdx.x);
+}
+// dW's tiles and dx's in one launch: they need nothing of each other, and
+// either alone often leaves part of the CUs without a tile (dW has few, long
+// ones, which come first).
+template <typename T, bool GROUPED, int KIND>
+__global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int nw, Args x) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if ((int)blockIdx.x < nw)
+        run_tile<T, true, true, GROUPED ? GROUP_RED : DENSE, KIND>(w, lds, blockIdx.x);
+    else
+        run_tile<T, false, true, GROUPED ? GROUP_ROWS : DENSE, KIND>(x, lds, blockIdx.x - nw);
 }
 
 // The slices' partial sums, added in their order (no atomics: the same result
@@ -933,7 +1068,7 @@ __global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
     float sum[W] = {};
     if (n > 0) {
         for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 32) {
-            float v[4][W], w[4][W];
+            float v[4][W], w[4][W] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int m = r + 8 * k < r1 && !tail ? n : 0;
@@ -942,9 +1077,7 @@ __global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (g.act != MDX_ACT_NONE && !tail)
-#pragma unroll
-                    for (int q = 0; q < W; ++q) v[k][q] = act_grad(v[k][q], w[k][q], g.act);
+                if (!tail) apply_act_grad(v[k], w[k], g.act);
                 if (g.dz && r + 8 * k < r1) store_row<T, W>(dz + (r + 8 * k) * g.lddz, n, v[k]);
 #pragma unroll
                 for (int q = 0; q < W; ++q) sum[q] += v[k][q];
@@ -1000,25 +1133,92 @@ __global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) {
 }
 
 // ---- host ---------------------------------------------------------------
-static long long ceil128(long long n) { return (n + 127) / 128; }
-
 // rows of a forward call that k_product_few takes (grouped: on average)
-constexpr int FEW = 64;
+constexpr int FEW = 32;
+constexpr int CUS = 256;  // of an MI355X
 
-// slices of the reduction: enough workgroups for two on each of the 256 CUs,
-// each of at least 4 steps of 128 bytes
-static int choose_splits(long long tiles, long long R, int es) {
-    const long long steps = (R * es + 127) / 128;
-    long long s = std::min<long long>(512 / std::max<long long>(tiles, 1), steps / 4);
-    return (int)std::max<long long>(1, std::min<long long>(s, 16));
+struct Shape {
+    long long T;  // rows
+    int E, N, K;  // E = 0: dense
+    int dtype, act;
+    int es() const { return dtype == 0 ? 4 : 2; }
+};
+
+// A product as the choice of kernel sees it: its output, the length of its
+// reduction, and how many of it there are (grouped: on average).
+struct Load {
+    long long I, J, R, groups;
+    bool red, split;  // grouped reduction; the reduction may be split
+};  // (of two, the first may be)
+struct Choice {
+    int kind, splits;  // splits of each load that may be split
+    double us;
+};
+// Microseconds of a step of 128 bytes for a tile alone on its CU, and for each
+// of several that share it; of a tile beside its steps; tiles that fit on a CU.
+// Measured on square layers of whole tiles (2048 x 2048, 1024 x 1024; reductions
+// of 512 and 4096).
+struct Cost {
+    double alone, shared, fixed;
+    int slots;
+};
+static Cost cost_of(int kind, int es) {
+    switch (kind) {
+        case LARGE: return {1.3, 1.3, 12.0, 1};
+        case DMA128: return es == 4 ? Cost{2.05, 1.9, 8.0, 2} : Cost{0.62, 0.62, 7.0, 1};
+        case DMA64: return es == 4 ? Cost{0.65, 0.55, 5.0, 2} : Cost{0.28, 0.175, 4.0, 2};
+        case REG128: return es == 4 ? Cost{2.2, 2.0, 8.0, 2} : Cost{1.2, 0.8, 5.0, 2};
+        default: return es == 4 ? Cost{0.8, 0.57, 5.0, 4} : Cost{0.6, 0.35, 3.5, 4};
+    }
 }
-static int fwd_splits(long long M, int N, int K, int dtype) {
-    if (M <= FEW) return 1;
-    return choose_splits(ceil128(M) * ceil128(N), K, dtype == 0 ? 4 : 2);
+// The kernel for one launch of all of `loads`, and the slices of their
+// reductions: the least estimate of the rounds in which the CUs work through
+// the tiles, and of the join.  (1000 x 1024 x 12544: fp32 128-wide tiles in 8
+// slices 205 us, in 4 216, 64-wide in 2 222; bf16 64-wide in 2 slices 46, 128-wide
+// in 4 47, 256-wide in 8 51.)
+static Choice choose(const Load *loads, int n, int es, bool aligned, long long most_part) {
+    Choice best{REG64, 1, 1e30};
+    for (int kind = aligned ? (es == 2 ? LARGE : DMA128) : REG128; kind <= (aligned ? DMA64 : REG64); ++kind) {
+        const Cost c = cost_of(kind, es);
+        const int side = tile_side(kind);
+        for (int splits = 1; splits <= 16; ++splits) {
+            double tiles[2], steps[2], all = 0, part = 0;
+            bool fits = true;
+            for (int k = 0; k < n; ++k) {
+                const Load &l = loads[k];
+                const int s = l.split ? splits : 1;
+                steps[k] = std::max(1.0, std::ceil((double)ceil_div(l.R * es, 128) / s));
+                if (s > 1 && steps[k] < 4) fits = false;
+                tiles[k] = (double)ceil_div(l.I, side) * ceil_div(l.J, side) * l.groups * s;
+                all += tiles[k];
+                if (s > 1) part += 4.0 * s * l.I * l.J * (l.red ? l.groups : 1);
+            }
+            if (!fits || part > most_part) break;
+            const double here = std::min((double)c.slots, std::max(1.0, std::ceil(all / CUS)));
+            const double step = std::max(c.alone, here * c.shared);
+            double work = 0, longest = 0;
+            for (int k = 0; k < n; ++k) {
+                work += tiles[k] * (steps[k] * step + c.fixed);
+                longest = std::max(longest, steps[k] * step + c.fixed);
+            }
+            const double rounds = std::max(1.0, std::ceil(work / (longest * CUS * here) - 0.02));
+            const double us = rounds * longest + (part > 0 ? 5.0 + part / 4e6 : 0.0);
+            if (us < 0.98 * best.us) best = Choice{kind, splits, us};
+            if (!loads[0].split) break;
+        }
+    }
+    return best;
 }
-static int dw_splits(int E, long long T, int N, int K, int dtype) {
-    return choose_splits((long long)E * ceil128(N) * ceil128(K), T / std::max(E, 1), dtype == 0 ? 4 : 2);
+static Load forward_load(const Shape &p) {
+    const long long E = std::max(p.E, 1);
+    return Load{ceil_div(p.T, E), p.N, p.K, E, false, p.E == 0};
 }
+// bytes of partial sums of a forward call; nothing in grouped ones is split
+static long long part_bytes(long long splits, long long E, long long I, long long J) {
+    return splits > 1 ? splits * std::max<long long>(E, 1) * I * J * 4 : 0;
+}
+constexpr long long PART_MAX = 1ll << 30;
+
 // rows of a chunk of k_act_backward: about eight workgroups for each CU
 static int act_rows(long long T, int N, int dtype) {
     const long long cols = ceil_div(N, dtype == 0 ? 128 : 256);
@@ -1029,69 +1229,64 @@ static long long act_chunks(int E, long long T, int rows) {
     return std::max<long long>(1, ceil_div(T, rows)) + (E ? E + 1 : 0);
 }
 
-// the large tile: both operands in whole aligned pieces of 16 bytes, and
-// enough tiles
-template <typename T, bool TA, bool TB> static bool use_big(const Args &g, int mode) {
-    if (sizeof(T) != 2) return false;
-    auto piece = [](const void *p, long long ld) {
-        return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(2 * ld)) % 16 == 0 && ld < (1ll << 22);
-    };
-    if (!piece(g.a, g.lda) || !piece(g.b, g.ldb) || g.gstride % 8) return false;
-    if ((TA ? g.I : g.R) % 8 || (TB ? g.J : g.R) % 8) return false;
-    const long long groups = mode == GROUP_RED ? g.E : 1;
-    return ceil_div(g.I, BIG) * ceil_div(g.J, BIG) * groups * g.splits >= 128;
+// whether an operand can be taken in aligned pieces of 16 bytes: r its
+// reduction (or its rows' length where that is i or j)
+static bool pieces(const void *p, long long ld, long long group, long long length, int es) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0 && group * es % 16 == 0 &&
+           length * es % 16 == 0 && ld < (1ll << 22);
 }
-// grid of tiles bi x bj; grouped rows: one partial tile more for each group,
-// and for the rows behind them; at most `most` workgroups
-constexpr int CUS = 256;  // of an MI355X; a multiple of its XCDs
-static int set_grid(Args &g, int mode, int bi, int bj, int threads, int most, dim3 &grid) {
+// tiles of a product as run in its launch; grouped rows: a bound, with one
+// partial tile more for each group and for the rows behind them
+static int set_tiles(Args &g, int mode, int bi, int bj, int threads, long long &n) {
     const long long ti = ceil_div(g.I, bi) + (mode == GROUP_ROWS ? g.E + 1 : 0), tj = ceil_div(g.J, bj);
-    const long long n = ti * tj * (mode == GROUP_RED ? g.E : 1) * g.splits;
-    MDX_REQUIRE(n < (1ll << 31) && std::min<long long>(n, most) * threads < (1ll << 32),
-                "mdx_linear: too many output tiles");
+    n = ti * tj * (mode == GROUP_RED ? g.E : 1) * g.splits;
+    MDX_REQUIRE(n * threads < (1ll << 31), "mdx_linear: too many output tiles");
     g.ti = (int)ti;
     g.tj = (int)tj;
-    grid = dim3((unsigned)std::min<long long>(n, most));
     return MDX_OK;
 }
-template <typename T, bool TA, bool TB, int MODE> static int launch_product(Args g, hipStream_t s) {
-    dim3 grid;
-    int rc = MDX_OK;
-    bool done = false;
-    if constexpr (sizeof(T) == 2) {
-        if (use_big<T, TA, TB>(g, MODE)) {
-            static const hipError_t attr = hipFuncSetAttribute(
-                reinterpret_cast<const void *>(k_product_big<T, TA, TB, MODE>),
-                hipFuncAttributeMaxDynamicSharedMemorySize, BIG_LDS);
-            MDX_HIP(attr);
-            if ((rc = set_grid(g, MODE, BIG, BIG, 512, INT32_MAX, grid))) return rc;
-            hipLaunchKernelGGL((k_product_big<T, TA, TB, MODE>), grid, dim3(512), BIG_LDS, s, g);
-            done = true;
-        }
-    }
-    const long long groups = MODE == GROUP_RED ? g.E : 1;
-    if (!done && ceil128(g.I) * ceil128(g.J) * groups * g.splits >= 256) {
-        if ((rc = set_grid(g, MODE, 128, 128, 256, INT32_MAX, grid))) return rc;
-        hipLaunchKernelGGL((k_product<T, TA, TB, MODE, 128>), grid, dim3(256), 0, s, g);
-    } else if (!done) {
-        if ((rc = set_grid(g, MODE, 64, 64, 256, INT32_MAX, grid))) return rc;
-        hipLaunchKernelGGL((k_product<T, TA, TB, MODE, 64>), grid, dim3(256), 0, s, g);
-    }
+template <typename T, bool GROUP> static int launch_join(const Args &g, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(g.I * ceil_div(g.J, VEC<T>), 256), GROUP ? g.E : 1);
+    hipLaunchKernelGGL(k_product_join<T>, grid, dim3(256), 0, s, g);
     MDX_CHECK_LAUNCH("mdx_linear");
-    if (g.splits > 1) {
-        const dim3 jg((unsigned)ceil_div(g.I * ceil_div(g.J, VEC<T>), 256), MODE == GROUP_RED ? g.E : 1);
-        hipLaunchKernelGGL(k_product_join<T>, jg, dim3(256), 0, s, g);
-        MDX_CHECK_LAUNCH("mdx_linear");
-    }
     return MDX_OK;
+}
+template <typename T, int MODE, int KIND> static int launch_forward(Args g, hipStream_t s) {
+    if constexpr (KIND == LARGE && sizeof(T) == 4) return MDX_EINVAL;
+    else {
+        long long n;
+        if (int rc = set_tiles(g, MODE, tile_side(KIND), tile_side(KIND), tile_threads(KIND), n)) return rc;
+        hipLaunchKernelGGL((k_forward<T, MODE, KIND>), dim3((unsigned)n), dim3(tile_threads(KIND)), tile_lds<T>(KIND), s,
+                           g);
+        MDX_CHECK_LAUNCH("mdx_linear");
+        return g.splits > 1 ? launch_join<T, false>(g, s) : MDX_OK;
+    }
+}
+// w, x: dW's and dx's product, their pointer out null where not needed
+template <typename T, bool GROUPED, int KIND> static int launch_backward(Args w, Args x, hipStream_t s) {
+    if constexpr (KIND == LARGE && sizeof(T) == 4) return MDX_EINVAL;
+    else {
+        long long nw = 0, nx = 0;
+        constexpr int side = tile_side(KIND), threads = tile_threads(KIND);
+        if (w.out)
+            if (int rc = set_tiles(w, GROUPED ? GROUP_RED : DENSE, side, side, threads, nw)) return rc;
+        if (x.out)
+            if (int rc = set_tiles(x, GROUPED ? GROUP_ROWS : DENSE, side, side, threads, nx)) return rc;
+        MDX_REQUIRE((nw + nx) * threads < (1ll << 31), "mdx_linear_backward: too many output tiles");
+        hipLaunchKernelGGL((k_backward<T, GROUPED, KIND>), dim3((unsigned)(nw + nx)), dim3(threads), tile_lds<T>(KIND), s,
+                           w, (int)nw, x);
+        MDX_CHECK_LAUNCH("mdx_linear_backward");
+        return w.out && w.splits > 1 ? launch_join<T, GROUPED>(w, s) : MDX_OK;
+    }
 }
 
-// few rows to a group: 16, 32 or 64 of them in a tile, 4, 8 or 16 waves to the reduction
+// few rows to a group: 16 or 32 of them in a tile, 4, 8 or 16 waves to the reduction
 template <typename T, int MODE, int MT> static int launch_few(Args g, hipStream_t s) {
     const long long chunks = ceil_div(g.R * (long long)sizeof(T), 128);
     const int waves = chunks >= 128 ? 16 : chunks >= 32 ? 8 : 4;
-    dim3 grid;
-    if (int rc = set_grid(g, MODE, 16 * MT, 16, 64 * waves, INT32_MAX, grid)) return rc;
+    long long n;
+    if (int rc = set_tiles(g, MODE, 16 * MT, 16, 64 * waves, n)) return rc;
+    const dim3 grid((unsigned)n);
     switch (waves) {
         case 16: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 16>), grid, dim3(1024), 0, s, g); break;
         case 8: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 8>), grid, dim3(512), 0, s, g); break;
@@ -1101,11 +1296,6 @@ template <typename T, int MODE, int MT> static int launch_few(Args g, hipStream_
     return MDX_OK;
 }
 
-struct Shape {
-    long long T;  // rows
-    int E, N, K;  // E = 0: dense
-    int dtype, act;
-};
 static int check_shape(const char *fn, const Shape &p) {
     MDX_REQUIRE(p.dtype == 0 || p.dtype == 1 || p.dtype == 3, "%s: dtype must be 0 (f32), 1 (f16) or 3 (bf16)", fn);
     MDX_REQUIRE(p.act >= MDX_ACT_NONE && p.act <= MDX_ACT_SILU, "%s: unknown activation %d", fn, p.act);
@@ -1115,15 +1305,34 @@ static int check_shape(const char *fn, const Shape &p) {
 }
 static bool bad_ld(const void *p, long long ld, long long width) { return p && ld < width; }
 
-template <typename T, int MODE> static int forward_mode(const Shape &p, const Args &g, hipStream_t s) {
-    const long long rows = ceil_div(p.T, std::max(p.E, 1));
-    if (rows <= 16) return launch_few<T, MODE, 1>(g, s);
-    if (rows <= 32) return launch_few<T, MODE, 2>(g, s);
-    if (rows <= FEW) return launch_few<T, MODE, 4>(g, s);
-    return launch_product<T, false, false, MODE>(g, s);
+static bool few_rows(const Shape &p) { return ceil_div(p.T, std::max(p.E, 1)) <= FEW; }
+template <typename T, int MODE> static int forward(const Shape &p, Args g, int64_t ws_bytes, hipStream_t s) {
+    g.splits = 1;
+    if (few_rows(p)) {
+        const long long rows = ceil_div(p.T, std::max(p.E, 1));
+        return rows <= 16 ? launch_few<T, MODE, 1>(g, s) : launch_few<T, MODE, 2>(g, s);
+    }
+    const int es = sizeof(T);
+    const Load l = forward_load(p);
+    const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
+    const Choice c = choose(&l, 1, es, al, g.part ? ws_bytes : 0);
+    g.splits = c.splits;
+    switch (c.kind) {
+        case LARGE: return launch_forward<T, MODE, LARGE>(g, s);
+        case DMA128: return launch_forward<T, MODE, DMA128>(g, s);
+        case DMA64: return launch_forward<T, MODE, DMA64>(g, s);
+        case REG128: return launch_forward<T, MODE, REG128>(g, s);
+        default: return launch_forward<T, MODE, REG64>(g, s);
+    }
 }
-template <typename T> static int forward(const Shape &p, const Args &g, hipStream_t s) {
-    return p.E ? forward_mode<T, GROUP_ROWS>(p, g, s) : forward_mode<T, DENSE>(p, g, s);
+// room for the split that either kind of kernel chooses, aligned operands or not
+static long long forward_bytes(const Shape &p) {
+    if (p.E || few_rows(p)) return 0;
+    const Load l = forward_load(p);
+    long long n = 0;
+    for (int al = 0; al < 2; ++al)
+        n = std::max(n, part_bytes(choose(&l, 1, p.es(), al, PART_MAX).splits, 0, p.T, p.N));
+    return n;
 }
 
 struct Back {
@@ -1138,93 +1347,111 @@ struct Back {
 };
 // workspace: dz | sums of db | partial dW, each 256-B aligned
 struct BackPlan {
-    bool sums, dz;  // the elementwise pass: for its sums, for dz in the workspace
-    int rows, splits;  // of a chunk of the elementwise pass; slices of dw's reduction
+    bool dz;           // dz is kept in the workspace
+    int rows;          // of a chunk of the elementwise pass
+    Choice products;
     long long dz_bytes, part_bytes, dw_bytes;
 };
 static long long up256(long long n) { return (n + 255) / 256 * 256; }
-static BackPlan plan_backward(const Shape &p, bool need_x, bool need_w, bool need_b, bool need_r) {
+static BackPlan plan_backward(const Shape &p, bool need_x, bool need_w, bool need_b, bool need_r, bool aligned) {
     BackPlan q{};
-    const int E = std::max(p.E, 1), es = p.dtype == 0 ? 4 : 2;
-    q.sums = need_b;
+    const long long E = std::max(p.E, 1);
+    // chosen for both products whichever are needed, so that a gradient's bits
+    // do not depend on which others are asked for
+    const Load l[2] = {Load{p.N, p.K, ceil_div(p.T, E), E, true, true},
+                       Load{ceil_div(p.T, E), p.K, p.N, E, false, false}};
+    q.products = choose(l, 2, p.es(), aligned, PART_MAX);
     q.dz = p.act != MDX_ACT_NONE && (need_x || need_w) && !need_r;
     q.rows = act_rows(p.T, p.N, p.dtype);
-    q.splits = need_w ? dw_splits(E, p.T, p.N, p.K, p.dtype) : 1;
-    q.dz_bytes = q.dz ? up256(p.T * p.N * es) : 0;
+    q.dz_bytes = q.dz ? up256(p.T * p.N * p.es()) : 0;
     q.part_bytes = need_b ? up256(act_chunks(p.E, p.T, q.rows) * p.N * 4) : 0;
-    q.dw_bytes = q.splits > 1 ? up256((long long)q.splits * E * p.N * p.K * 4) : 0;
+    q.dw_bytes = need_w ? up256(part_bytes(q.products.splits, p.E, p.N, p.K)) : 0;
     return q;
 }
+// room for what either kind of kernel chooses, aligned operands or not
+static long long backward_bytes(const Shape &p, bool need_x, bool need_w, bool need_b, bool need_r) {
+    long long n = 0;
+    for (int al = 0; al < 2; ++al) {
+        const BackPlan q = plan_backward(p, need_x, need_w, need_b, need_r, al);
+        n = std::max(n, q.dz_bytes + q.part_bytes + q.dw_bytes);
+    }
+    return n;
+}
 
-template <typename T> static int backward(const Shape &p, const Back &b, hipStream_t s) {
-    const BackPlan q = plan_backward(p, b.dx, b.dw, b.db, b.dres);
-    const int E = std::max(p.E, 1);
-    const void *dz = b.grad;
-    long long lddz = b.ldg;
-    float *part = reinterpret_cast<float *>(b.ws + q.dz_bytes);
+template <typename T, bool GROUPED> static int backward(const Shape &p, const Back &b, hipStream_t s) {
+    const int E = std::max(p.E, 1), es = sizeof(T);
+    // dz as the products take it; its rows in the workspace lie N apart
+    const bool kept = p.act != MDX_ACT_NONE;
+    const void *dz = !kept ? b.grad : b.dres ? b.dres : b.ws;
+    const long long lddz = !kept ? b.ldg : b.dres ? b.lddr : p.N;
+    const bool al = pieces(dz, lddz, 0, p.N, es) && pieces(b.x, b.ldx, 0, p.K, es) &&
+                    pieces(b.w, b.ldw, (long long)p.N * b.ldw, p.K, es);
+    const BackPlan q = plan_backward(p, b.dx, b.dw, b.db, b.dres, al);
     if (q.dz || b.db || b.dres) {
         ActArgs a{};
         a.dy = b.grad; a.ldy = b.ldg;
         a.z = b.pre; a.ldz = b.ldp;
         a.dz = b.dres ? b.dres : q.dz ? b.ws : nullptr;
         a.lddz = b.dres ? b.lddr : p.N;
-        a.part = b.db ? part : nullptr;
+        a.part = b.db ? reinterpret_cast<float *>(b.ws + q.dz_bytes) : nullptr;
         a.counts = b.counts;
         a.E = p.E; a.T = p.T; a.N = p.N; a.act = p.act;
         a.rows = q.rows;
         a.zero_tail = b.dres && b.zero_tail;
-        const long long chunks = act_chunks(p.E, p.T, q.rows);
-        const dim3 grid((unsigned)ceil_div(p.N, 32 * VEC<T>), (unsigned)chunks);
+        const dim3 grid((unsigned)ceil_div(p.N, 32 * VEC<T>), (unsigned)act_chunks(p.E, p.T, q.rows));
         hipLaunchKernelGGL(k_act_backward<T>, grid, dim3(256), 0, s, a);
         MDX_CHECK_LAUNCH("mdx_linear_backward");
         if (b.db) {
             hipLaunchKernelGGL(k_bias_join, dim3((unsigned)ceil_div(p.N, 16), E), dim3(256), 0, s, a, b.db);
             MDX_CHECK_LAUNCH("mdx_linear_backward");
         }
-        if (a.dz && p.act != MDX_ACT_NONE) {
-            dz = a.dz;
-            lddz = a.lddz;
-        }
+    }
+    Args w{}, x{};
+    w.splits = x.splits = 1;
+    if (b.dw) {
+        w.a = dz; w.lda = lddz;
+        w.b = b.x; w.ldb = b.ldx;
+        w.I = p.N; w.J = p.K; w.R = p.T;
+        w.out = b.dw; w.ldo = b.lddw;
+        w.counts = b.counts; w.E = p.E; w.T = p.T;
+        w.gstride = (long long)p.N * b.lddw;
+        w.splits = q.products.splits;
+        w.part = reinterpret_cast<float *>(b.ws + q.dz_bytes + q.part_bytes);
     }
     if (b.dx && p.T) {
-        Args g{};
-        g.a = dz; g.lda = lddz;
-        g.b = b.w; g.ldb = b.ldw;
-        g.I = p.T; g.J = p.K; g.R = p.N;
-        g.out = b.dx; g.ldo = b.lddx;
-        g.counts = b.counts; g.E = p.E; g.T = p.T;
-        g.gstride = (long long)p.N * b.ldw;
-        g.zero_tail = b.zero_tail;
-        g.splits = 1;
-        const int rc = p.E ? launch_product<T, false, true, GROUP_ROWS>(g, s)
-                           : launch_product<T, false, true, DENSE>(g, s);
-        if (rc != MDX_OK) return rc;
+        x.a = dz; x.lda = lddz;
+        x.b = b.w; x.ldb = b.ldw;
+        x.I = p.T; x.J = p.K; x.R = p.N;
+        x.out = b.dx; x.ldo = b.lddx;
+        x.counts = b.counts; x.E = p.E; x.T = p.T;
+        x.gstride = (long long)p.N * b.ldw;
+        x.zero_tail = b.zero_tail;
     }
-    if (b.dw) {
-        Args g{};
-        g.a = dz; g.lda = lddz;
-        g.b = b.x; g.ldb = b.ldx;
-        g.I = p.N; g.J = p.K; g.R = p.T;
-        g.out = b.dw; g.ldo = b.lddw;
-        g.counts = b.counts; g.E = p.E; g.T = p.T;
-        g.gstride = (long long)p.N * b.lddw;
-        g.splits = q.splits;
-        g.part = reinterpret_cast<float *>(b.ws + q.dz_bytes + q.part_bytes);
-        const int rc = p.E ? launch_product<T, true, true, GROUP_RED>(g, s) : launch_product<T, true, true, DENSE>(g, s);
-        if (rc != MDX_OK) return rc;
+    if (!w.out && !x.out) return MDX_OK;
+    switch (q.products.kind) {
+        case LARGE: return launch_backward<T, GROUPED, LARGE>(w, x, s);
+        case DMA128: return launch_backward<T, GROUPED, DMA128>(w, x, s);
+        case DMA64: return launch_backward<T, GROUPED, DMA64>(w, x, s);
+        case REG128: return launch_backward<T, GROUPED, REG128>(w, x, s);
+        default: return launch_backward<T, GROUPED, REG64>(w, x, s);
     }
-    return MDX_OK;
 }
 
-static int run_forward(const char *fn, const Shape &p, const Args &g, hipStream_t s) {
+template <typename T> static int forward_any(const Shape &p, const Args &g, int64_t ws_bytes, hipStream_t s) {
+    return p.E ? forward<T, GROUP_ROWS>(p, g, ws_bytes, s) : forward<T, DENSE>(p, g, ws_bytes, s);
+}
+template <typename T> static int backward_any(const Shape &p, const Back &b, hipStream_t s) {
+    return p.E ? backward<T, true>(p, b, s) : backward<T, false>(p, b, s);
+}
+static int run_forward(const char *fn, const Shape &p, const Args &g, int64_t ws_bytes, hipStream_t s) {
     MDX_REQUIRE(g.a && g.b && g.out, "%s: null pointer", fn);
     MDX_REQUIRE(!bad_ld(g.a, g.lda, p.K) && !bad_ld(g.b, g.ldb, p.K) && !bad_ld(g.res, g.ldr, p.N) &&
                     !bad_ld(g.pre, g.ldp, p.N) && !bad_ld(g.out, g.ldo, p.N),
                 "%s: a row stride is below its row's length", fn);
     switch (p.dtype) {
-        case 0: return forward<float>(p, g, s);
-        case 1: return forward<_Float16>(p, g, s);
-        default: return forward<__bf16>(p, g, s);
+        case 0: return forward_any<float>(p, g, ws_bytes, s);
+        case 1: return forward_any<_Float16>(p, g, ws_bytes, s);
+        default: return forward_any<__bf16>(p, g, ws_bytes, s);
     }
 }
 static int run_backward(const char *fn, const Shape &p, const Back &b, int64_t ws_bytes, hipStream_t s) {
@@ -1238,14 +1465,13 @@ static int run_backward(const char *fn, const Shape &p, const Back &b, int64_t w
                     !bad_ld(b.pre, b.ldp, p.N) && !bad_ld(b.dx, b.lddx, p.K) && !bad_ld(b.dw, b.lddw, p.K) &&
                     !bad_ld(b.dres, b.lddr, p.N),
                 "%s: a row stride is below its row's length", fn);
-    const BackPlan q = plan_backward(p, b.dx, b.dw, b.db, b.dres);
-    const long long need = q.dz_bytes + q.part_bytes + q.dw_bytes;
+    const long long need = backward_bytes(p, b.dx, b.dw, b.db, b.dres);
     MDX_REQUIRE(need == 0 || (b.ws && ws_bytes >= need), "%s: needs %lld bytes of workspace, got %lld", fn, need,
                 (long long)ws_bytes);
     switch (p.dtype) {
-        case 0: return backward<float>(p, b, s);
-        case 1: return backward<_Float16>(p, b, s);
-        default: return backward<__bf16>(p, b, s);
+        case 0: return backward_any<float>(p, b, s);
+        case 1: return backward_any<_Float16>(p, b, s);
+        default: return backward_any<__bf16>(p, b, s);
     }
 }
 
@@ -1257,8 +1483,7 @@ using namespace mdx::lin;
 
 extern "C" int64_t mdx_linear_workspace_bytes(int64_t M, int N, int K, int dtype) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const int s = fwd_splits(M, N, K, dtype);
-    return s > 1 ? (int64_t)s * M * N * 4 : 0;
+    return forward_bytes(Shape{M, 0, N, K, dtype, 0});
 }
 extern "C" int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *bias,
                           const void *residual, int64_t ldr, int64_t M, int N, int K, int act, int dtype, void *pre,
@@ -1276,17 +1501,14 @@ extern "C" int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw
     g.pre = pre; g.ldp = ldp;
     g.out = out; g.ldo = ldo;
     g.act = act;
-    g.splits = fwd_splits(M, N, K, dtype);
     g.part = reinterpret_cast<float *>(workspace);
-    if (!workspace || workspace_bytes < (int64_t)g.splits * M * N * 4) g.splits = 1;
-    return run_forward("mdx_linear", p, g, as_stream(stream));
+    return run_forward("mdx_linear", p, g, workspace_bytes, as_stream(stream));
 }
 
 extern "C" int64_t mdx_linear_backward_workspace_bytes(int64_t M, int N, int K, int act, int dtype, int need_x,
                                                        int need_w, int need_bias, int need_residual) {
     if (M < 0 || N <= 0 || K <= 0) return 0;
-    const BackPlan q = plan_backward(Shape{M, 0, N, K, dtype, act}, need_x, need_w, need_bias, need_residual);
-    return q.dz_bytes + q.part_bytes + q.dw_bytes;
+    return backward_bytes(Shape{M, 0, N, K, dtype, act}, need_x, need_w, need_bias, need_residual);
 }
 extern "C" int mdx_linear_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const void *w,
                                    int64_t ldw, const void *pre, int64_t ldp, int64_t M, int N, int K, int act,
@@ -1326,16 +1548,14 @@ extern "C" int mdx_grouped_linear(const void *x, int64_t ldx, const void *w, con
     g.counts = counts; g.E = E; g.T = T;
     g.gstride = (long long)N * K;
     g.zero_tail = zero_tail;
-    g.splits = 1;
-    return run_forward("mdx_grouped_linear", p, g, as_stream(stream));
+    return run_forward("mdx_grouped_linear", p, g, 0, as_stream(stream));
 }
 
 extern "C" int64_t mdx_grouped_linear_backward_workspace_bytes(int E, int64_t T, int N, int K, int act, int dtype,
                                                                int need_x, int need_w, int need_bias,
                                                                int need_residual) {
     if (E <= 0 || T < 0 || N <= 0 || K <= 0) return 0;
-    const BackPlan q = plan_backward(Shape{T, E, N, K, dtype, act}, need_x, need_w, need_bias, need_residual);
-    return q.dz_bytes + q.part_bytes + q.dw_bytes;
+    return backward_bytes(Shape{T, E, N, K, dtype, act}, need_x, need_w, need_bias, need_residual);
 }
 extern "C" int mdx_grouped_linear_backward(const void *grad, int64_t ldg, const void *x, int64_t ldx, const void *w,
                                            const void *pre, int64_t ldp, const int *counts, int E, int64_t T, int N,

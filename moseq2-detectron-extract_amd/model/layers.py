@@ -23,7 +23,6 @@ refused outside ``torch.no_grad()``, since no graph is recorded.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
@@ -53,12 +52,30 @@ class LayerNormGrads(NamedTuple):
 # ---------------------------------------------------------------------------
 # plumbing
 # ---------------------------------------------------------------------------
+# A call on a few rows takes the GPU some 5 us, so what a call costs on the
+# host counts: plain integers for pointers, the current stream's handle without
+# a Stream object, and a device guard only where another device is current.
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
-def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+def _stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _on:
+    """The device guard of a call: nothing where `device` is current."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _activation(name) -> int:
@@ -97,7 +114,15 @@ def _check_input(what: str, x: torch.Tensor, dims: int = 1) -> None:
 
 
 def _check_run(x: torch.Tensor, *others) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *others)):
+    if torch.is_grad_enabled():
+        for t in (x, *others):
+            if t is not None and t.requires_grad:
+                break
+        else:
+            t = None
+    else:
+        t = None
+    if t is not None:
         raise ValueError("a tensor requires grad: call under torch.no_grad() and take the gradients with the "
                          "_backward function (no autograd graph is recorded)")
     if not x.is_cuda:
@@ -109,6 +134,10 @@ def _rows(t: torch.Tensor, copy: bool = True) -> Optional[torch.Tensor]:
     distance of at least the width; a copy where its layout allows no such
     view (None with copy=False)."""
     width = t.shape[-1]
+    if t.is_contiguous():
+        r = t if t.dim() == 2 else t.view(-1, width)
+        if r.stride(0) == width:
+            return r
     n = t.numel() // width
     if n == 0:
         return t.reshape(0, width)
@@ -147,7 +176,7 @@ def _output(out: Optional[torch.Tensor], shape, like: torch.Tensor, reads, inpla
     must not share memory with `reads`, nor in part with `inplace`."""
     if out is None:
         out = torch.empty(shape, dtype=like.dtype, device=like.device)
-        return out, out.view(-1, shape[-1])
+        return out, out if len(shape) == 2 else out.view(-1, shape[-1])
     rows = _rows(out, copy=False)
     if rows is None:
         raise ValueError("out must have rows of unit stride at a constant distance")
@@ -232,7 +261,7 @@ def _forward(x, counts, weight, bias, residual, activation, return_pre, out):
         _check_counts(counts, E, x)
     _limits(x.numel() // K, N, K)
     _check_run(x, weight, bias, residual, out)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         xr = _rows(x)
         w = weight.contiguous() if grouped else _rows(weight)
         b = bias.contiguous() if bias is not None else None
@@ -250,12 +279,12 @@ def _forward(x, counts, weight, bias, residual, activation, return_pre, out):
                 if return_pre and not fresh:
                     pre.zero_()
                 call("mdx_grouped_linear", _ptr(xr), _ld(xr), _ptr(w), _ptr(b), _ptr(r), _ld(r), _ptr(counts), E, M, N,
-                     K, act, dt, _ptr(p), _ld(p), _ptr(o), _ld(o), int(fresh), _stream())
+                     K, act, dt, _ptr(p), _ld(p), _ptr(o), _ld(o), int(fresh), _stream(x.device))
             else:
                 nbytes = call("mdx_linear_workspace_bytes", M, N, K, dt)
                 ws = _workspace(nbytes, x.device)
                 call("mdx_linear", _ptr(xr), _ld(xr), _ptr(w), _ld(w), _ptr(b), _ptr(r), _ld(r), M, N, K, act, dt,
-                     _ptr(p), _ld(p), _ptr(o), _ld(o), _ptr(ws), nbytes, _stream())
+                     _ptr(p), _ld(p), _ptr(o), _ld(o), _ptr(ws), nbytes, _stream(x.device))
     return (out, pre) if return_pre else out
 
 
@@ -298,7 +327,7 @@ def _backward(grad, x, counts, weight, pre, activation, need_x, need_weight, nee
     _limits(x.numel() // K, N, K)
     _check_run(x, grad, weight, pre)
     dev = x.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         xr, gr = _rows(x), _rows(grad)
         w = weight.contiguous() if grouped else _rows(weight)
         z = _rows(pre) if act else None
@@ -318,12 +347,12 @@ def _backward(grad, x, counts, weight, pre, activation, need_x, need_weight, nee
                 ws = _workspace(nbytes, dev)
                 call("mdx_grouped_linear_backward", _ptr(gr), _ld(gr), _ptr(xr), _ld(xr), _ptr(w), _ptr(z), _ld(z),
                      _ptr(counts), E, M, N, K, act, dt, _ptr(dxr), K, _ptr(dw), _ptr(db), _ptr(drr), N, 1, _ptr(ws),
-                     nbytes, _stream())
+                     nbytes, _stream(x.device))
             else:
                 nbytes = call("mdx_linear_backward_workspace_bytes", M, N, K, act, dt, *flags)
                 ws = _workspace(nbytes, dev)
                 call("mdx_linear_backward", _ptr(gr), _ld(gr), _ptr(xr), _ld(xr), _ptr(w), _ld(w), _ptr(z), _ld(z), M,
-                     N, K, act, dt, _ptr(dxr), K, _ptr(dw), K, _ptr(db), _ptr(drr), N, _ptr(ws), nbytes, _stream())
+                     N, K, act, dt, _ptr(dxr), K, _ptr(dw), K, _ptr(db), _ptr(drr), N, _ptr(ws), nbytes, _stream(x.device))
     return LinearGrads(dx, dw, db, (dr if own else grad) if need_residual else None)
 
 
@@ -344,7 +373,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, return_stats: bo
         raise ValueError("eps must not be negative")
     _limits(0, D)
     _check_run(x, weight, bias, out)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         xr = _rows(x)
         w, b = (None if t is None else t.contiguous() for t in (weight, bias))
         out, o = _output(out, tuple(x.shape), x, [None if t is None else t.view(1, -1) for t in (w, b)], (xr,))
@@ -352,7 +381,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, return_stats: bo
                       for _ in range(2))
         if xr.shape[0]:
             call("mdx_layer_norm", _ptr(xr), _ld(xr), _ptr(w), _ptr(b), xr.shape[0], D, float(eps), _DTYPES[x.dtype],
-                 _ptr(o), _ld(o), _ptr(mean), _ptr(rstd), _stream())
+                 _ptr(o), _ld(o), _ptr(mean), _ptr(rstd), _stream(x.device))
     return (out, mean, rstd) if return_stats else out
 
 
@@ -372,7 +401,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, need_x: bool = True
     _limits(0, D)
     _check_run(x, grad, mean, rstd, weight)
     dev = x.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         xr, gr = _rows(x), _rows(grad)
         m, r = mean.contiguous(), rstd.contiguous()
         w = weight.contiguous() if weight is not None else None
@@ -384,5 +413,5 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, need_x: bool = True
             nbytes = call("mdx_layer_norm_backward_workspace_bytes", n, D, dt) if need_weight or need_bias else 0
             ws = _workspace(nbytes, dev)
             call("mdx_layer_norm_backward", _ptr(gr), _ld(gr), _ptr(xr), _ld(xr), _ptr(m), _ptr(r), _ptr(w), n, D, dt,
-                 _ptr(dx.view(-1, D) if need_x else None), D, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream())
+                 _ptr(dx.view(-1, D) if need_x else None), D, _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(x.device))
     return LayerNormGrads(dx, dw, db)

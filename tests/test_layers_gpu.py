@@ -638,3 +638,64 @@ def test_c_entry_with_less_workspace(L, mdx):
         check_forward(out, None, x.cpu(), w.cpu(), None, None, "none", F32)
         if nbytes < n:
             assert (ws == 255).all()
+
+
+# Shapes of whole and ragged large tiles (256 x 256, 16-bit, aligned rows):
+# reductions shorter than the pipeline's four steps of 64, of a whole number of
+# steps and not, odd and even numbers of them; grouped ones with short, empty
+# and long groups
+LARGE = [(4096, 2048, 8), (4104, 2048, 64), (4097, 2056, 136), (2048, 4096, 200), (8200, 1032, 256), (4096, 2048, 328),
+         (2300, 4104, 72), (4096, 2048, 648)]
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_tiles(L, dt, shape):
+    """Forward and backward where the 256-wide tile has enough work."""
+    M, N, K = shape
+    g = gen(M + N + K)
+    x, w, b = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, N)
+    r, dy, z = (normal(g, M, N, dtype=dt) for _ in range(3))
+    act = ACTS[1 + (M + K) % 4]
+    y, pre = L.linear(x.cuda(), w.cuda(), b.cuda(), r.cuda(), act, return_pre=True)
+    check_forward(y, pre, x, w, b, r, act, dt)
+    got = L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z.cuda(), act, need_bias=True, need_residual=True)
+    check_backward(got, dy, x, w, z, act, dt)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("E,N,K,counts,tail", [
+    (6, 2048, 72, [1000, 0, 3, 2000, 256, 700], 100), (3, 4096, 264, [1, 2000, 513], 0),
+    (9, 1032, 1024, [300, 0, 0, 900, 1300, 17, 0, 2100, 64], 900), (2, 2048, 128, [0, 4096], 1)])
+def test_large_tiles_grouped(L, dt, E, N, K, counts, tail):
+    T = sum(counts) + tail
+    x, w, b, z, dy = grouped_inputs(T, E, N, K, dt, T + N)
+    sp, end = spans(counts, T)
+    for t in (x, z, dy):
+        t[end:] = float("nan")
+    cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    act = ACTS[1 + T % 4]
+    y = L.grouped_linear(x.cuda(), cd, w.cuda(), b.cuda(), None, act)
+    got = L.grouped_linear_backward(dy.cuda(), x.cuda(), cd, w.cuda(), z.cuda(), act, need_bias=True, need_residual=True)
+    for e, (s, t) in enumerate(sp):
+        check_forward(y[s:t], None, x[s:t], w[e], b[e], None, act, dt)
+        check_backward(L_grads(got, e, s, t), dy[s:t], x[s:t], w[e], z[s:t], act, dt)
+    assert (y[end:] == 0).all() and (got.x[end:] == 0).all() and (got.residual[end:] == 0).all()
+    out = torch.full((T, N), 3.0, dtype=dt, device="cuda")
+    L.grouped_linear(x.cuda(), cd, w.cuda(), b.cuda(), None, act, out=out)
+    assert torch.equal(out[:end], y[:end]) and (out[end:] == 3).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(1000, 1024, 1024), (1000, 512, 4096), (2048, 1024, 72), (515, 1040, 2056),
+                                   (1001, 515, 1003), (2100, 1031, 263)])
+def test_middle_sizes(L, dt, M, N, K):
+    """The 64- and 128-wide tiles with whole and split reductions, aligned and not."""
+    g = gen(M + N + K)
+    x, w, b = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, N)
+    dy, z = normal(g, M, N, dtype=dt), normal(g, M, N, dtype=dt)
+    act = ACTS[(M + K) % 5]
+    y, pre = L.linear(x.cuda(), w.cuda(), b.cuda(), None, act, return_pre=True)
+    check_forward(y, pre, x, w, b, None, act, dt)
+    got = L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z.cuda(), act, need_bias=True, need_residual=True)
+    check_backward(got, dy, x, w, z, act, dt)
