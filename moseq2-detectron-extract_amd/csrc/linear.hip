@@ -196,80 +196,80 @@ struct Args {
 
 enum { DENSE = 0, GROUP_ROWS = 1, GROUP_RED = 2 };
 
-// a value that is the same in all lanes, and lane l's value, in scalar registers
+// a value that is the same in all lanes, in scalar registers
 __device__ __forceinline__ long long uniform(long long v) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
     return (long long)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | lo);
 }
-__device__ __forceinline__ long long lane_value(long long v, int l) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, l);
-    return (long long)((uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), l) << 32 | lo);
+// inclusive scan of v over the wave, every partial sum cut at most (below
+// 2^31), so that no count makes it wrap; lane shifts in the ALU (DPP)
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t v, uint32_t most) {
+    return min(v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false), most);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t most) {
+    v = dpp_add<0x111, 0xf>(v, most);  // row_shr 1, 2, 4, 8: rows of 16 lanes
+    v = dpp_add<0x112, 0xf>(v, most);
+    v = dpp_add<0x114, 0xf>(v, most);
+    v = dpp_add<0x118, 0xf>(v, most);
+    v = dpp_add<0x142, 0xa>(v, most);  // row_bcast 15, 31: the rows before
+    return dpp_add<0x143, 0xc>(v, most);
 }
 
 struct Span {
-    int e;                 // group, E = the rows behind the last one, -1 = none
-    long long start, end;  // its rows
-    long long tile, tile0; // tile within the group; the group's first tile
+    int e;           // group, E = the rows behind the last one, -1 = none
+    int start, end;  // its rows
+    int tile, tile0; // tile within the group; the group's first tile
 };
-
-// The group holding tile `tile` when each group's rows are cut into tiles of
-// bm (want < 0), or group `want` itself (E: the rows behind the last one).
-// Every wave scans the counts 64 at a time with its lanes, so no pass over the
-// counts has to run before.
-__device__ __forceinline__ Span find_group(const int *counts, int E, long long T, int bm, long long tile, int want) {
-    const int lane = threadIdx.x & 63;
-    long long row0 = 0, tile0 = 0;
-    for (int base = 0; base < E; base += 64) {
-        const long long c = base + lane < E ? max(counts[base + lane], 0) : 0;
-        long long rows = c;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long v = __shfl_up(rows, d);
-            if (lane >= d) rows += v;
-        }
-        const long long s = min(row0 + rows - c, T), e = min(row0 + rows, T), mine = (e - s + bm - 1) / bm;
-        long long tiles = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long v = __shfl_up(tiles, d);
-            if (lane >= d) tiles += v;
-        }
-        const long long t1 = tile0 + tiles, t0 = t1 - mine;
-        const unsigned long long hit =
-            __ballot(base + lane < E && (want >= 0 ? base + lane == want : tile >= t0 && tile < t1));
-        if (hit) {
-            const int l = __ffsll(hit) - 1;
-            const long long first = lane_value(t0, l);
-            return Span{base + l, lane_value(s, l), lane_value(e, l), tile - first, first};
-        }
-        row0 = min(row0 + lane_value(rows, 63), T);
-        tile0 = lane_value(t1, 63);
+// 64 groups at once, a lane each: their rows start .. end, cut at T, and their
+// first tiles of bm rows.  Every wave that needs a group scans the counts
+// itself, so no pass over them has to run before.
+struct Groups {
+    uint32_t start, end, tile0, tiles;  // of the lane's group
+    uint32_t rows, next;                // behind the last of the 64: rows, tiles
+    __device__ __forceinline__ Groups(const int *counts, int E, long long T, int bm, int base, uint32_t rows0,
+                                      uint32_t first) {
+        const int lane = threadIdx.x & 63;
+        const uint32_t t = (uint32_t)T, c = base + lane < E ? min((uint32_t)max(counts[base + lane], 0), t) : 0;
+        const uint32_t sum = wave_scan(c, t), before = (uint32_t)__shfl_up((int)sum, 1);  // with all lanes active
+        end = min(rows0 + sum, t);
+        start = min(rows0 + (lane ? before : 0u), t);
+        tiles = (end - start + bm - 1) / bm;
+        const uint32_t all = wave_scan(tiles, 0x7fffffffu);
+        tile0 = first + all - tiles;
+        rows = __builtin_amdgcn_readlane(end, 63);
+        next = first + __builtin_amdgcn_readlane(all, 63);
     }
-    if (want >= 0 ? want == E : row0 < T && tile < tile0 + (T - row0 + bm - 1) / bm)
-        return Span{E, row0, T, tile - tile0, tile0};
-    return Span{-1, 0, 0, 0, 0};
+    __device__ __forceinline__ Span span(unsigned long long hit, int base, int tile) const {
+        const int l = __ffsll(hit) - 1, t0 = (int)__builtin_amdgcn_readlane(tile0, l);
+        return Span{base + l, (int)__builtin_amdgcn_readlane(start, l), (int)__builtin_amdgcn_readlane(end, l),
+                    tile - t0, t0};
+    }
+    __device__ __forceinline__ unsigned long long holds(int tile) const {
+        return __ballot((uint32_t)tile >= tile0 && (uint32_t)tile < tile0 + tiles);
+    }
+};
+// group `want` (below E), its rows cut into tiles of bm
+__device__ __forceinline__ Span find_group(const int *counts, int E, long long T, int bm, int want) {
+    uint32_t rows = 0, next = 0;
+    for (int base = 0;; base += 64) {
+        const Groups g(counts, E, T, bm, base, rows, next);
+        if (want < base + 64) return g.span(1ull << (want - base), base, 0);
+        rows = g.rows;
+        next = g.next;
+    }
 }
-
-// tiles of bm rows of all groups; *rows: the rows that they hold together
-__device__ __forceinline__ long long count_tiles(const int *counts, int E, long long T, int bm, long long *rows) {
-    const int lane = threadIdx.x & 63;
-    long long row0 = 0, n = 0;
+// the group that holds tile `tile`, or the rows behind the last one (e = E), or none
+__device__ __forceinline__ Span find_tile(const int *counts, int E, long long T, int bm, int tile) {
+    uint32_t rows = 0, next = 0;
     for (int base = 0; base < E; base += 64) {
-        const long long c = base + lane < E ? max(counts[base + lane], 0) : 0;
-        long long r = c;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long v = __shfl_up(r, d);
-            if (lane >= d) r += v;
-        }
-        long long mine = (min(row0 + r, T) - min(row0 + r - c, T) + bm - 1) / bm;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
-        n += uniform(mine);
-        row0 = min(row0 + lane_value(r, 63), T);
+        const Groups g(counts, E, T, bm, base, rows, next);
+        if (const unsigned long long hit = g.holds(tile)) return g.span(hit, base, tile);
+        rows = g.rows;
+        next = g.next;
     }
-    *rows = row0;
-    return n;
+    if (rows < (uint32_t)T && tile < (int)(next + ((uint32_t)T - rows + bm - 1) / bm))
+        return Span{E, (int)rows, (int)T, tile - (int)next, (int)next};
+    return Span{-1, 0, 0, 0, 0};
 }
 
 // tile id of ti x tj -> (row tile, column tile): contiguous ranges of tiles for
@@ -283,39 +283,44 @@ __device__ __forceinline__ void map_tile(unsigned id, unsigned ti, unsigned tj, 
     u = in / rows;
 }
 
-// the tiles of a product: ids 0 .. n - 1
-struct Work {
-    int n, ti;       // row tiles that hold rows
-    long long rows;  // grouped rows: rows of all groups
-};
-template <int MODE> __device__ __forceinline__ Work list_work(const Args &g, int bi) {
-    Work k{g.ti * g.tj * g.splits, g.ti, g.I};
-    if (MODE == GROUP_RED) k.n *= g.E;
-    if (MODE == GROUP_ROWS) {  // g.ti is a bound
-        k.ti = (int)count_tiles(g.counts, g.E, g.T, bi, &k.rows);
-        k.n = (k.ti + (g.zero_tail ? (int)((g.T - k.rows + bi - 1) / bi) : 0)) * g.tj;
-    }
-    return k;
-}
-// One of them: rows i0 .. of i1, columns from j0, the reduction r0 .. r1, and
-// the offsets of its group and slice.
+// What a workgroup computes: rows i0 .. of i1, columns from j0, the reduction
+// r0 .. r1, and the offsets of its group and slice.
 struct Where {
     long long i0, i1, r0, r1, boff, biasoff, ooff;
     int j0, grp;  // grp: place of its partial sums
     bool tail;    // rows behind the last group: zeros
 };
-template <int MODE>
-__device__ __forceinline__ Where locate(const Args &g, const Work &k, int id, int bi, int bj, int bk) {
-    Where w{0, g.I, 0, g.R, 0, 0, 0, 0, 0, false};
+// tile id of a product in tiles of bi x bj, its slices in steps of bk; false:
+// there is none (the grid of grouped rows is a bound)
+template <int MODE> __device__ __forceinline__ bool place(const Args &g, int id, int bi, int bj, int bk, Where &w) {
+    w = Where{0, g.I, 0, g.R, 0, 0, 0, 0, 0, false};
     int t, u;
-    if (MODE == GROUP_ROWS && id >= k.ti * g.tj) {  // the rows behind come last, so that the XCDs' ranges are even
-        id -= k.ti * g.tj;
-        w.i0 = k.rows + (long long)(id / g.tj) * bi;
-        w.i1 = g.T;
-        w.j0 = id % g.tj * bj;
-        w.r1 = 0;
-        w.tail = true;
-        return w;
+    if (MODE == GROUP_ROWS) {
+        const Groups first(g.counts, g.E, g.T, bi, 0, 0, 0);
+        uint32_t rows = first.rows, tiles = first.next;
+        for (int base = 64; base < g.E; base += 64) {
+            const Groups k(g.counts, g.E, g.T, bi, base, rows, tiles);
+            rows = k.rows;
+            tiles = k.next;
+        }
+        if (id >= (int)tiles * g.tj) {  // the rows behind come last, so that the XCDs' ranges are even
+            id -= (int)tiles * g.tj;
+            w.i0 = (long long)rows + (long long)(id / g.tj) * bi;
+            w.i1 = g.T;
+            w.j0 = id % g.tj * bj;
+            w.r1 = 0;
+            w.tail = true;
+            return g.zero_tail && w.i0 < g.T;
+        }
+        map_tile(id, tiles, g.tj, t, u);
+        const unsigned long long hit = first.holds(t);
+        const Span s = hit ? first.span(hit, 0, t) : find_tile(g.counts, g.E, g.T, bi, t);
+        w.i0 = s.start + (long long)bi * s.tile;
+        w.i1 = s.end;
+        w.boff = s.e * g.gstride;
+        w.biasoff = (long long)s.e * g.J;
+        w.j0 = bj * u;
+        return true;
     }
     int e = 0, z = 0;
     if (MODE == GROUP_RED || g.splits > 1) {
@@ -328,18 +333,11 @@ __device__ __forceinline__ Where locate(const Args &g, const Work &k, int id, in
             e = w.grp - z * g.E;
         }
     }
-    map_tile(id, k.ti, g.tj, t, u);
+    map_tile(id, g.ti, g.tj, t, u);
     w.i0 = (long long)bi * t;
     w.j0 = bj * u;
-    if (MODE == GROUP_ROWS) {
-        const Span s = find_group(g.counts, g.E, g.T, bi, t, -1);
-        w.i0 = s.start + bi * s.tile;
-        w.i1 = s.end;
-        w.boff = s.e * g.gstride;
-        w.biasoff = (long long)s.e * g.J;
-    }
     if (MODE == GROUP_RED) {
-        const Span s = find_group(g.counts, g.E, g.T, 1, 0, e);
+        const Span s = find_group(g.counts, g.E, g.T, 1, e);
         w.r0 = s.start;
         w.r1 = s.end;
         w.ooff = e * g.gstride;
@@ -349,7 +347,7 @@ __device__ __forceinline__ Where locate(const Args &g, const Work &k, int id, in
         w.r0 = min(w.r1, w.r0 + (long long)z * per * bk);
         w.r1 = min(w.r1, w.r0 + (long long)per * bk);
     }
-    return w;
+    return true;
 }
 
 // 16 bytes of a row of outputs from their sums v: bias b (zeros if there is
@@ -626,9 +624,8 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
     constexpr int Q = SIDE / 2, N = Q / 16;  // a wave's quarter, its MFMA tiles each way
     constexpr int STEP = SA::BYTES + SB::BYTES, NB = BUFS<T, SIDE, DMA>;
     static_assert(4 * epi_bytes(Q) <= 2 * STEP, "the epilogue takes the operands' LDS");
-    const Work work = list_work<MODE>(g, SIDE);
-    if (id >= work.n) return;
-    const Where w = locate<MODE>(g, work, id, SIDE, SIDE, SA::BK);
+    Where w;
+    if (!place<MODE>(g, id, SIDE, SIDE, SA::BK, w)) return;
     const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b) + w.boff;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = (wid >> 1) * Q, wj = (wid & 1) * Q;
     f4 acc[N][N];
@@ -718,69 +715,87 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
 
 // ---- few rows -----------------------------------------------------------
 // x of at most a few rows (or groups of them) against a wide weight: what
-// counts is to stream the weight.  A workgroup takes 16 columns by 16 MT rows;
-// its waves share the reduction, each wave 128 bytes of every row at a time
-// (lane: row l & 15, two pieces at 32 (l >> 4) bytes), four such chunks in
-// flight, straight from memory into the MFMAs; the waves' sums meet in LDS.
-// Rows and columns beyond the end are clamped: their products are not stored.
-template <typename T, int MODE, int MT, int WAVES>
+// counts is to stream the weight.  A workgroup takes 16 NT columns by 16 MT
+// rows; its waves share the reduction (or its slice), each wave 128 bytes of
+// every row at a time (lane: row l & 15, two pieces at 32 (l >> 4) bytes), four
+// such chunks in flight, straight from memory into the MFMAs; the waves' sums
+// meet in LDS.  Rows and columns beyond the end are clamped: their products are
+// not stored.
+template <typename T, int MODE, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
-    constexpr int N = VEC<T>, KC = 8 * N, U = 4, ROWS = 16 * MT;
-    __shared__ __attribute__((aligned(16))) float red[WAVES][ROWS][16];
-    const Work work = list_work<MODE>(g, ROWS);
-    if ((int)blockIdx.x >= work.n) return;
-    const Where w = locate<MODE>(g, work, blockIdx.x, ROWS, 16, 1);
+    constexpr int N = VEC<T>, KC = 8 * N, U = 4, ROWS = 16 * MT, COLS = 16 * NT;
+    __shared__ __attribute__((aligned(16))) float red[WAVES][ROWS][COLS];
+    Where w;
+    if (!place<MODE>(g, blockIdx.x, ROWS, COLS, KC, w)) return;
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, f = lane & 15, q = lane >> 4;
-    const T *B = reinterpret_cast<const T *>(g.b) + w.boff + min(w.j0 + f, g.J - 1) * g.ldb;
-    const T *A[MT];
+    const T *A[MT], *B[NT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) A[m] = reinterpret_cast<const T *>(g.a) + min(w.i0 + 16 * m + f, w.i1 - 1) * g.lda;
-    f4 acc[MT];
+    for (int n = 0; n < NT; ++n)
+        B[n] = reinterpret_cast<const T *>(g.b) + w.boff + min(w.j0 + 16 * n + f, g.J - 1) * g.ldb + w.r0;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = f4{0.f, 0.f, 0.f, 0.f};
-    const int K = (int)w.r1, whole = K / KC;
+    for (int m = 0; m < MT; ++m)
+        A[m] = reinterpret_cast<const T *>(g.a) + min(w.i0 + 16 * m + f, w.i1 - 1) * g.lda + w.r0;
+    f4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
+    const int K = (int)(w.r1 - w.r0), whole = K / KC, r0 = (int)w.r0;
     if (!w.tail) {
         int c = wid;
         for (; c + (U - 1) * WAVES < whole; c += U * WAVES) {
-            u4 b[U][2];
+            u4 b[U][NT][2];
 #pragma unroll
             for (int k = 0; k < U; ++k)
 #pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    b[k][p] = reinterpret_cast<const Un16<T> *>(B + (c + k * WAVES) * KC + (2 * q + p) * N)->v;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        b[k][n][p] = reinterpret_cast<const Un16<T> *>(B[n] + (c + k * WAVES) * KC + (2 * q + p) * N)->v;
 #pragma unroll
             for (int k = 0; k < U; ++k)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        acc[m] = Mma<T>::mul(
-                            b[k][p],
-                            reinterpret_cast<const Un16<T> *>(A[m] + (c + k * WAVES) * KC + (2 * q + p) * N)->v, acc[m]);
+                    for (int p = 0; p < 2; ++p) {
+                        const u4 a =
+                            reinterpret_cast<const Un16<T> *>(A[m] + (c + k * WAVES) * KC + (2 * q + p) * N)->v;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[m][n] = Mma<T>::mul(b[k][n][p], a, acc[m][n]);
+                    }
         }
         for (; c * KC < K; c += WAVES)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const int k = c * KC + (2 * q + p) * N;
-                const u4 b = load_piece(B + k, k, K - k);
+                u4 b[NT];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) acc[m] = Mma<T>::mul(b, load_piece(A[m] + k, k, K - k), acc[m]);
+                for (int n = 0; n < NT; ++n) b[n] = load_piece(B[n] + k, r0 + k, K - k);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const u4 a = load_piece(A[m] + k, r0 + k, K - k);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[m][n] = Mma<T>::mul(b[n], a, acc[m][n]);
+                }
             }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) *reinterpret_cast<f4 *>(&red[wid][16 * m + f][4 * q]) = acc[m];
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<f4 *>(&red[wid][16 * m + f][16 * n + 4 * q]) = acc[m][n];
     __syncthreads();
-    for (int t = threadIdx.x; t < ROWS * 16 / N; t += 64 * WAVES) {
-        const int r = t / (16 / N), c = t % (16 / N) * N;
+    for (int t = threadIdx.x; t < ROWS * COLS / N; t += 64 * WAVES) {
+        const int r = t / (COLS / N), c = t % (COLS / N) * N;
         if (w.i0 + r >= w.i1 || w.j0 + c >= g.J) continue;
-        float v[N] = {};
+        const u4 res = g.splits == 1 && !w.tail ? load_residual<T>(g, w.i0 + r, w.j0 + c) : u4{0, 0, 0, 0};
+        float v[N] = {}, b[N] = {};
+        if (g.bias && g.splits == 1 && !w.tail)
+            load_row<float, N>(g.bias + w.biasoff + w.j0 + c, w.j0 + c, g.J - w.j0 - c, b);
 #pragma unroll
         for (int k = 0; k < WAVES; ++k)
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] += red[k][r][c + e];
-        float b[N] = {};
-        if (g.bias && !w.tail) load_row<float, N>(g.bias + w.biasoff + w.j0 + c, w.j0 + c, g.J - w.j0 - c, b);
-        store_outputs<T>(g, w, w.i0 + r, w.j0 + c, v, b, load_residual<T>(g, w.i0 + r, w.j0 + c));
+        store_outputs<T>(g, w, w.i0 + r, w.j0 + c, v, b, res);
     }
 }
 
@@ -858,9 +873,8 @@ template <typename T, bool TR, bool ISB> struct BigOperand {
 // 5 to 45 % slower than a workgroup per tile.)
 template <typename T, bool TA, bool TB, int MODE>
 __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
-    const Work work = list_work<MODE>(g, BIG);
-    if (id >= work.n) return;
-    const Where w = locate<MODE>(g, work, id, BIG, BIG, 64);
+    Where w;
+    if (!place<MODE>(g, id, BIG, BIG, 64, w)) return;
     using std::integral_constant;
     constexpr integral_constant<int, 0> c0{};
     constexpr integral_constant<int, 1> c1{};
@@ -1056,11 +1070,11 @@ __global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
     long long r0 = (long long)blockIdx.y * g.rows, r1 = min(g.T, r0 + g.rows);
     bool tail = false;
     if (g.counts) {
-        const Span s = find_group(g.counts, g.E, g.T, g.rows, blockIdx.y, -1);
+        const Span s = find_tile(g.counts, g.E, g.T, g.rows, blockIdx.y);
         tail = s.e == g.E;
         if (s.e < 0 || (tail && !g.zero_tail)) return;
-        r0 = s.start + s.tile * g.rows;
-        r1 = min(s.end, r0 + g.rows);
+        r0 = s.start + (long long)s.tile * g.rows;
+        r1 = min((long long)s.end, r0 + g.rows);
     }
     const int c = (blockIdx.x * 32 + (threadIdx.x & 31)) * W, n = g.N - c;
     const T *dy = reinterpret_cast<const T *>(g.dy) + c, *z = reinterpret_cast<const T *>(g.z) + c;
@@ -1105,7 +1119,7 @@ __global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) {
     const int l = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + l;
     long long first = 0, n = (g.T + g.rows - 1) / g.rows;
     if (g.counts) {
-        const Span s = find_group(g.counts, g.E, g.T, g.rows, 0, blockIdx.y);
+        const Span s = find_group(g.counts, g.E, g.T, g.rows, blockIdx.y);
         first = s.tile0;
         n = (s.end - s.start + g.rows - 1) / g.rows;
     }
@@ -1280,20 +1294,34 @@ template <typename T, bool GROUPED, int KIND> static int launch_backward(Args w,
     }
 }
 
-// few rows to a group: 16 or 32 of them in a tile, 4, 8 or 16 waves to the reduction
-template <typename T, int MODE, int MT> static int launch_few(Args g, hipStream_t s) {
-    const long long chunks = ceil_div(g.R * (long long)sizeof(T), 128);
-    const int waves = chunks >= 128 ? 16 : chunks >= 32 ? 8 : 4;
+// Few rows to a group: 16 or 32 of them in a tile; 32 columns where that still
+// gives every CU a few workgroups, else 16 and slices of the reduction until
+// every CU has one; 4, 8 or 16 waves to a slice of it.
+struct Few {
+    int mt, nt, splits, waves;
+};
+static Few few_plan(long long rows, int E, long long N, long long K, int es) {
+    Few f{rows <= 16 ? 1 : 2, 1, 1, 4};
+    const long long chunks = ceil_div(K * es, 128), live = std::max(E, 1);
+    if (ceil_div(N, 32) * live >= 4 * CUS) f.nt = 2;
+    const long long tiles = ceil_div(N, 16 * f.nt) * live;
+    if (!E) f.splits = (int)std::max<long long>(1, std::min<long long>(std::min(CUS / tiles, chunks / 32), 8));
+    const long long each = ceil_div(chunks, f.splits);
+    f.waves = each >= 64 && tiles * f.splits <= 2 * CUS ? 16 : each >= 32 ? 8 : 4;
+    return f;
+}
+template <typename T, bool GROUP> static int launch_join(const Args &g, hipStream_t s);
+template <typename T, int MODE, int MT, int NT> static int launch_few(Args g, int waves, hipStream_t s) {
     long long n;
-    if (int rc = set_tiles(g, MODE, 16 * MT, 16, 64 * waves, n)) return rc;
+    if (int rc = set_tiles(g, MODE, 16 * MT, 16 * NT, 64 * waves, n)) return rc;
     const dim3 grid((unsigned)n);
     switch (waves) {
-        case 16: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 16>), grid, dim3(1024), 0, s, g); break;
-        case 8: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 8>), grid, dim3(512), 0, s, g); break;
-        default: hipLaunchKernelGGL((k_product_few<T, MODE, MT, 4>), grid, dim3(256), 0, s, g);
+        case 16: hipLaunchKernelGGL((k_product_few<T, MODE, MT, NT, 16>), grid, dim3(1024), 0, s, g); break;
+        case 8: hipLaunchKernelGGL((k_product_few<T, MODE, MT, NT, 8>), grid, dim3(512), 0, s, g); break;
+        default: hipLaunchKernelGGL((k_product_few<T, MODE, MT, NT, 4>), grid, dim3(256), 0, s, g);
     }
     MDX_CHECK_LAUNCH("mdx_linear");
-    return MDX_OK;
+    return g.splits > 1 ? launch_join<T, false>(g, s) : MDX_OK;
 }
 
 static int check_shape(const char *fn, const Shape &p) {
@@ -1308,11 +1336,14 @@ static bool bad_ld(const void *p, long long ld, long long width) { return p && l
 static bool few_rows(const Shape &p) { return ceil_div(p.T, std::max(p.E, 1)) <= FEW; }
 template <typename T, int MODE> static int forward(const Shape &p, Args g, int64_t ws_bytes, hipStream_t s) {
     g.splits = 1;
-    if (few_rows(p)) {
-        const long long rows = ceil_div(p.T, std::max(p.E, 1));
-        return rows <= 16 ? launch_few<T, MODE, 1>(g, s) : launch_few<T, MODE, 2>(g, s);
-    }
     const int es = sizeof(T);
+    if (few_rows(p)) {
+        const Few f = few_plan(ceil_div(p.T, std::max(p.E, 1)), p.E, p.N, p.K, es);
+        if (f.splits > 1 && g.part && ws_bytes >= part_bytes(f.splits, 0, p.T, p.N)) g.splits = f.splits;
+        if (f.mt == 1)
+            return f.nt == 1 ? launch_few<T, MODE, 1, 1>(g, f.waves, s) : launch_few<T, MODE, 1, 2>(g, f.waves, s);
+        return f.nt == 1 ? launch_few<T, MODE, 2, 1>(g, f.waves, s) : launch_few<T, MODE, 2, 2>(g, f.waves, s);
+    }
     const Load l = forward_load(p);
     const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
     const Choice c = choose(&l, 1, es, al, g.part ? ws_bytes : 0);
@@ -1327,7 +1358,8 @@ template <typename T, int MODE> static int forward(const Shape &p, Args g, int64
 }
 // room for the split that either kind of kernel chooses, aligned operands or not
 static long long forward_bytes(const Shape &p) {
-    if (p.E || few_rows(p)) return 0;
+    if (p.E) return 0;
+    if (few_rows(p)) return part_bytes(few_plan(p.T, 0, p.N, p.K, p.es()).splits, 0, p.T, p.N);
     const Load l = forward_load(p);
     long long n = 0;
     for (int al = 0; al < 2; ++al)

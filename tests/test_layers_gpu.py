@@ -699,3 +699,40 @@ def test_middle_sizes(L, dt, M, N, K):
     check_forward(y, pre, x, w, b, None, act, dt)
     got = L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z.cuda(), act, need_bias=True, need_residual=True)
     check_backward(got, dy, x, w, z, act, dt)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("M", [1, 5, 16, 17, 32])
+@pytest.mark.parametrize("N,K", [(1024, 12544), (40, 8200), (4100, 264), (2056, 4100), (30, 4099), (33000, 16)])
+def test_few_rows(L, dt, M, N, K):
+    """Few rows: long reductions in slices, wide weights, odd ends of both."""
+    g = gen(M + N + K)
+    x, w, b, r = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, N), normal(g, M, N, dtype=dt)
+    act = ACTS[(M + K) % 5]
+    y, pre = L.linear(strided(x, 3, 1), w.cuda(), b.cuda(), r.cuda(), act, return_pre=True)
+    check_forward(y, pre, x, w, b, r, act, dt)
+
+
+def many_counts(E, g):
+    c = torch.randint(0, 4, (E,), generator=g)
+    c[torch.randperm(E, generator=g)[:E // 3]] = 0
+    c[E // 2] = 300
+    return c.tolist()
+
+
+@pytest.mark.parametrize("E", [63, 64, 65, 200, 1000])
+def test_many_groups(L, E):
+    """More groups than a wave has lanes, and the edges of that."""
+    g = gen(E)
+    counts = many_counts(E, g)
+    T, N, K, dt = sum(counts) + 3, 24, 40, BF16
+    x, w, b, z, dy = grouped_inputs(T, E, N, K, dt, E)
+    sp, end = spans(counts, T)
+    cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    y = L.grouped_linear(x.cuda(), cd, w.cuda(), b.cuda(), None, "silu")
+    got = L.grouped_linear_backward(dy.cuda(), x.cuda(), cd, w.cuda(), z.cuda(), "silu", need_bias=True, need_residual=True)
+    y, got = y.cpu(), type(got)(*(t.cpu() for t in got))
+    for e, (s, t) in enumerate(sp):
+        check_forward(y[s:t], None, x[s:t], w[e], b[e], None, "silu", dt)
+        check_backward(L_grads(got, e, s, t), dy[s:t], x[s:t], w[e], z[s:t], "silu", dt)
+    assert (y[end:] == 0).all() and (got.x[end:] == 0).all()
