@@ -32,29 +32,32 @@ template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Un16 { 
 
 template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 
+// 16 bytes shifted down by s bits, 0 <= s < 128
+__device__ __forceinline__ u4 shift_down(u4 v, int s) {
+    union { u4 u; unsigned long long d[2]; } r;
+    r.u = v;
+    if (s >= 64) {
+        r.d[0] = r.d[1];
+        r.d[1] = 0;
+        s -= 64;
+    }
+    if (s) {
+        r.d[0] = r.d[0] >> s | r.d[1] << (64 - s);
+        r.d[1] >>= s;
+    }
+    return r.u;
+}
 // 16 bytes of a row from its element c on, of which the first n exist (n <= 0:
 // none); the rest is zero.  The last piece of a row is read as the 16 bytes
 // that end with it, shifted down.
 template <typename T> __device__ __forceinline__ u4 load_piece(const T *p, long long c, long long n) {
     constexpr int N = VEC<T>;
     if (n >= N) return reinterpret_cast<const Un16<T> *>(p)->v;
-    union { u4 u; unsigned long long d[2]; T e[N]; } r;
+    if (n <= 0) return u4{0, 0, 0, 0};
+    if (c + n >= N)
+        return shift_down(reinterpret_cast<const Un16<T> *>(p - (N - n))->v, (int)(N - n) * 8 * (int)sizeof(T));
+    union { u4 u; T e[N]; } r;
     r.u = u4{0, 0, 0, 0};
-    if (n <= 0) return r.u;
-    if (c + n >= N) {
-        r.u = reinterpret_cast<const Un16<T> *>(p - (N - n))->v;
-        int s = (int)(N - n) * 8 * (int)sizeof(T);
-        if (s >= 64) {
-            r.d[0] = r.d[1];
-            r.d[1] = 0;
-            s -= 64;
-        }
-        if (s) {
-            r.d[0] = r.d[0] >> s | r.d[1] << (64 - s);
-            r.d[1] >>= s;
-        }
-        return r.u;
-    }
 #pragma unroll
     for (int q = 0; q < N; ++q)
         if (q < n) r.e[q] = p[q];
@@ -496,25 +499,6 @@ template <typename T, bool TR, int SIDE> struct Stage {
         if (SIDE == 64) return (((row >> 1) & 1) | (((row >> 3) & 1) << 1)) << 1;  // two rows to all banks
         return ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
     }
-    // the thread's pieces of the tile whose first i is i0 and first r is r0
-    static __device__ __forceinline__ void load(const T *p, long long ld, long long i0, long long I, long long r0,
-                                                long long R, u4 (&v)[N]) {
-        const int pc = threadIdx.x % PPR, row = threadIdx.x / PPR;
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const long long w = (TR ? r0 : i0) + row + STEP * q, c = (TR ? i0 : r0) + pc * VEC<T>;
-            const long long left = w < (TR ? R : I) ? (TR ? I : R) - c : 0;
-            v[q] = load_piece(left > 0 ? p + w * ld + c : p, c, left);
-        }
-    }
-    static __device__ __forceinline__ void write(char *lds, const u4 (&v)[N]) {
-        const int pc = threadIdx.x % PPR, row = threadIdx.x / PPR;
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const int r = row + STEP * q;
-            *reinterpret_cast<u4 *>(lds + r * PITCH + ((pc ^ swz(r)) << 4)) = v[q];
-        }
-    }
     // fragment of rows i0 .. i0 + 15, 64-B step s
     static __device__ __forceinline__ u4 frag(const char *lds, int i0, int s) {
         const int lane = threadIdx.x & 63, f = lane & 15, q = lane >> 4;
@@ -535,6 +519,74 @@ template <typename T, bool TR, int SIDE> struct Stage {
 #pragma unroll
             for (int e = 0; e < 4; ++e) r[e] = *reinterpret_cast<const uint32_t *>(p + e * PITCH);
             return r;
+        }
+    }
+};
+
+// A thread's part in staging one operand of any alignment through registers:
+// its N pieces of a step.  load() brings 16 bytes for each, of the row's end
+// where the piece passes it and of anything near where there is no piece;
+// write() puts that right on the way to LDS, so that no load is waited for
+// before.  Rows shorter than a piece are finished in load() (`tiny`).
+template <typename T, bool TR, int SIDE> struct RegOperand {
+    using S = Stage<T, TR, SIDE>;
+    static constexpr int N = S::N, V = VEC<T>;
+    const T *row[N];  // TR 0: the piece's row; TR 1: the piece in its row of the next step
+    const T *base;    // TR 1: a piece that can always be read
+    long long step;
+    int at, end, r0, left;  // TR 0: the piece's first r, the reduction's end; TR 1: its row of the next step, the end
+    bool in[N], tiny;       // TR 0: the row exists; TR 1: (left: elements of the piece's row from its first on)
+    __device__ __forceinline__ void init(const T *p, long long ld, long long i0, long long I, long long r0_, long long R) {
+        const int t = threadIdx.x, pc = t % S::PPR;
+        tiny = (TR ? I : R) < V;
+        end = (int)R;
+        step = S::BK * ld;
+        if (TR) {
+            const int c = (int)i0 + pc * V;
+            at = (int)r0_ + t / S::PPR;
+            left = (int)I - c;
+            base = p + (tiny ? (left > 0 ? c : 0) : min(c, (int)I - V));
+#pragma unroll
+            for (int q = 0; q < N; ++q) row[q] = base + (long long)(at + S::STEP * q) * ld;
+        } else {
+            at = (int)r0_ + pc * V;
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const long long w = i0 + t / S::PPR + S::STEP * q;
+                in[q] = w < I;
+                row[q] = p + min(w, I - 1) * ld;
+            }
+        }
+    }
+    // the next step's pieces
+    __device__ __forceinline__ void load(u4 (&v)[N]) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            if (TR) {
+                const bool live = at + S::STEP * q < end;
+                if (tiny)
+                    v[q] = load_piece(row[q], 0, live ? left : 0);
+                else
+                    v[q] = reinterpret_cast<const Un16<T> *>(live ? row[q] : base)->v;
+                row[q] += step;
+            } else if (tiny) {
+                v[q] = load_piece(row[q] + (at < end ? at : 0), at, in[q] ? end - at : 0);
+            } else {
+                v[q] = reinterpret_cast<const Un16<T> *>(row[q] + min(at, end - V))->v;
+            }
+        }
+        at += S::BK;
+    }
+    // the pieces that load() brought `back` steps ago
+    __device__ __forceinline__ void write(char *lds, int back, const u4 (&v)[N]) const {
+        const int pc = threadIdx.x % S::PPR, first = threadIdx.x / S::PPR, was = at - back * S::BK;
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const int r = first + S::STEP * q;
+            const int n = TR ? (was + S::STEP * q < end ? left : 0) : in[q] ? end - was : 0;
+            u4 u = v[q];
+            if (!tiny && n < V) u = n > 0 ? shift_down(u, (V - n) * 8 * (int)sizeof(T)) : u4{0, 0, 0, 0};
+            *reinterpret_cast<u4 *>(lds + r * S::PITCH + ((pc ^ S::swz(r)) << 4)) = u;
         }
     }
 };
@@ -579,7 +631,7 @@ __device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t 
 // BUFS - 1 steps ahead, so that a lone workgroup on a CU does not wait out the
 // memory's latency at each step; one barrier a step, behind which step s has
 // landed everywhere and step s - 1 has been read, so that its buffer is free.
-// Otherwise: any alignment and sizes, through registers, one step ahead.
+// Otherwise: any alignment and sizes, through registers, two or three steps ahead.
 template <typename T, int SIDE, bool DMA> constexpr int BUFS = !DMA || (sizeof(T) == 4 && SIDE == 128) ? 2 : 4;
 
 // a lane's part in staging one operand by DMA: instruction d of wave w brings
@@ -678,27 +730,34 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
             dma_wait<0>();  // nothing may land in the epilogue's LDS
         }
     } else {
-        u4 va[SA::N], vb[SB::N];
+        constexpr int AHEAD = SIDE == 64 ? 3 : 2;
+        RegOperand<T, TA, SIDE> oa;
+        RegOperand<T, TB, SIDE> ob;
+        u4 va[AHEAD][SA::N], vb[AHEAD][SB::N];
         if (steps > 0) {
-            SA::load(A, g.lda, w.i0, w.i1, w.r0, w.r1, va);
-            SB::load(B, g.ldb, w.j0, g.J, w.r0, w.r1, vb);
-            SA::write(lds, va);
-            SB::write(lds + SA::BYTES, vb);
-        }
-        for (long long s = 0; s < steps; ++s) {
-            __syncthreads();
-            if (s + 1 < steps) {
-                SA::load(A, g.lda, w.i0, w.i1, w.r0 + (s + 1) * SA::BK, w.r1, va);
-                SB::load(B, g.ldb, w.j0, g.J, w.r0 + (s + 1) * SA::BK, w.r1, vb);
-            }
-            u4 fa[2][N], fb[2][N];
-            read(fa, fb, lds + (s & 1) * STEP);
-            multiply(fa, fb);
-            if (s + 1 < steps) {
-                SA::write(lds + ((s + 1) & 1) * STEP, va);
-                SB::write(lds + ((s + 1) & 1) * STEP + SA::BYTES, vb);
+            oa.init(A, g.lda, w.i0, w.i1, w.r0, w.r1);
+            ob.init(B, g.ldb, w.j0, g.J, w.r0, w.r1);
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) {
+                oa.load(va[d]);
+                ob.load(vb[d]);
             }
         }
+        for (int s0 = 0; s0 < (int)steps; s0 += AHEAD)
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) {
+                const int s = s0 + d;
+                if (s >= (int)steps) break;
+                char *l = lds + (s & 1) * STEP;  // last read at step s - 2, before the barrier of step s - 1
+                oa.write(l, AHEAD, va[d]);
+                ob.write(l + SA::BYTES, AHEAD, vb[d]);
+                oa.load(va[d]);
+                ob.load(vb[d]);
+                __syncthreads();
+                u4 fa[2][N], fb[2][N];
+                read(fa, fb, l);
+                multiply(fa, fb);
+            }
     }
     __syncthreads();  // the operands' buffers become the epilogue's
     epilogue<T, Q, N>(
@@ -1051,7 +1110,7 @@ __global__ __launch_bounds__(256) void k_product_join(Args g) {
 // dz = dy act'(z) in T, and the column sums of dz before that rounding.  A
 // workgroup takes one chunk of `rows` rows of a group by 32 pieces of 16 bytes;
 // its sums go to part[chunk][N], and k_bias_join adds a group's chunks.  Bound
-// by HBM: four rows of each thread are in flight at once.
+// by HBM.
 struct ActArgs {
     const void *dy, *z;
     long long ldy, ldz;
@@ -1065,8 +1124,8 @@ struct ActArgs {
     int zero_tail;       // write zeros to dz behind the last group
 };
 template <typename T>
-__global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
-    constexpr int W = VEC<T>;
+__global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
+    constexpr int W = VEC<T>, AT = 2;  // rows of a thread at once
     long long r0 = (long long)blockIdx.y * g.rows, r1 = min(g.T, r0 + g.rows);
     bool tail = false;
     if (g.counts) {
@@ -1081,16 +1140,16 @@ __global__ __launch_bounds__(256) void k_act_backward(ActArgs g) {
     T *dz = reinterpret_cast<T *>(g.dz) + c;
     float sum[W] = {};
     if (n > 0) {
-        for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 32) {
-            float v[4][W], w[4][W] = {};
+        for (long long r = r0 + (threadIdx.x >> 5); r < r1; r += 8 * AT) {
+            float v[AT][W], w[AT][W] = {};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < AT; ++k) {
                 const int m = r + 8 * k < r1 && !tail ? n : 0;
                 load_row<T, W>(dy + (m ? (r + 8 * k) * g.ldy : 0), c, m, v[k]);
                 if (g.act != MDX_ACT_NONE) load_row<T, W>(z + (m ? (r + 8 * k) * g.ldz : 0), c, m, w[k]);
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < AT; ++k) {
                 if (!tail) apply_act_grad(v[k], w[k], g.act);
                 if (g.dz && r + 8 * k < r1) store_row<T, W>(dz + (r + 8 * k) * g.lddz, n, v[k]);
 #pragma unroll
@@ -1327,7 +1386,9 @@ template <typename T, int MODE, int MT, int NT> static int launch_few(Args g, in
 static int check_shape(const char *fn, const Shape &p) {
     MDX_REQUIRE(p.dtype == 0 || p.dtype == 1 || p.dtype == 3, "%s: dtype must be 0 (f32), 1 (f16) or 3 (bf16)", fn);
     MDX_REQUIRE(p.act >= MDX_ACT_NONE && p.act <= MDX_ACT_SILU, "%s: unknown activation %d", fn, p.act);
-    MDX_REQUIRE(p.T >= 0 && p.T < (1ll << 31) && p.N > 0 && p.K > 0, "%s: bad shape", fn);
+    // positions in a row or column, and a few steps behind them, are 32-bit
+    constexpr int most = INT32_MAX - (1 << 16);
+    MDX_REQUIRE(p.T >= 0 && p.T <= most && p.N > 0 && p.N <= most && p.K > 0 && p.K <= most, "%s: bad shape", fn);
     MDX_REQUIRE(p.E >= 0 && p.E <= 4096, "%s: 1 to 4096 groups", fn);
     return MDX_OK;
 }

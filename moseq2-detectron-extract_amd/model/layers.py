@@ -31,7 +31,7 @@ from .._lib import call
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3}
-_I32_MAX = 2 ** 31 - 1
+_MOST = 2 ** 31 - 1 - 2 ** 16  # rows, columns
 
 
 class LinearGrads(NamedTuple):
@@ -199,8 +199,8 @@ def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
 
 
 def _limits(rows: int, *widths: int) -> None:
-    if rows > _I32_MAX or any(w > _I32_MAX for w in widths):
-        raise ValueError("sizes must be below 2^31")
+    if rows > _MOST or any(w > _MOST for w in widths):
+        raise ValueError(f"at most {_MOST} rows and columns")
 
 
 def _check_counts(counts, E: int, like: torch.Tensor) -> None:
