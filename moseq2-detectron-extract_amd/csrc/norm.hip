@@ -23,17 +23,35 @@ template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
 template <typename T> struct Piece {
     union { u4 u; T e[VEC<T>]; };
 };
-// the piece at p, of which the first n elements exist (n <= 0: none); the rest is 0
-template <typename T> __device__ __forceinline__ Piece<T> load(const T *p, int n) {
-    Piece<T> r;
-    if (n >= VEC<T>) {
-        r.u = reinterpret_cast<const Un16<T> *>(p)->v;
-        return r;
+// 16 bytes shifted down by s bits, 0 <= s < 128
+__device__ __forceinline__ u4 shift_down(u4 v, int s) {
+    union { u4 u; unsigned long long d[2]; } r;
+    r.u = v;
+    if (s >= 64) {
+        r.d[0] = r.d[1];
+        r.d[1] = 0;
+        s -= 64;
     }
+    if (s) {
+        r.d[0] = r.d[0] >> s | r.d[1] << (64 - s);
+        r.d[1] >>= s;
+    }
+    return r.u;
+}
+// the piece at a row's element c, of which the first n elements exist (n <= 0:
+// none); the rest is 0.  The last piece of a row is read as the 16 bytes that
+// end with it, shifted down.
+template <typename T> __device__ __forceinline__ Piece<T> load(const T *p, int c, int n) {
+    Piece<T> r;
     r.u = u4{0, 0, 0, 0};
+    if (n >= VEC<T>)
+        r.u = reinterpret_cast<const Un16<T> *>(p)->v;
+    else if (n > 0 && c + n >= VEC<T>)
+        r.u = shift_down(reinterpret_cast<const Un16<T> *>(p - (VEC<T> - n))->v, (VEC<T> - n) * 8 * (int)sizeof(T));
+    else
 #pragma unroll
-    for (int q = 0; q < VEC<T>; ++q)
-        if (q < n) r.e[q] = p[q];
+        for (int q = 0; q < VEC<T>; ++q)
+            if (q < n) r.e[q] = p[q];
     return r;
 }
 template <typename T> __device__ __forceinline__ void store(T *p, const Piece<T> &v, int n) {
@@ -59,79 +77,139 @@ struct Args {
     float *part;                // backward: [workgroups][2][D] partial dg, db, or null
 };
 
-// sum over the TPR threads of a row (TPR <= 64: lanes of a wave; above: the
-// workgroup, through LDS).  Every thread gets it.
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float *sh) {
+// Sums over the TPR threads of a row (TPR <= 64: lanes of a wave; above: the
+// workgroup, through LDS), which every thread gets.  Within 16 lanes the adds
+// take their operand from another lane directly (DPP); N sums go side by side,
+// so that their latencies overlap.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int TPR, int N> __device__ __forceinline__ void row_sums(float (&v)[N], float *sh) {
 #pragma unroll
-    for (int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+    for (int k = 0; k < N; ++k) {
+        v[k] = dpp_add<0xB1>(v[k]);   // lanes 1, 0, 3, 2 of each four
+        v[k] = dpp_add<0x4E>(v[k]);   // 2, 3, 0, 1
+        v[k] = dpp_add<0x141>(v[k]);  // mirrored in 8
+        v[k] = dpp_add<0x140>(v[k]);  // mirrored in 16
+    }
+#pragma unroll
+    for (int d = 16; d < (TPR < 64 ? TPR : 64); d <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], d);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
-        __syncthreads();  // the sums before this one have been read
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
+        __syncthreads();  // the sums before these have been read
+        if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += sh[w];
+            for (int k = 0; k < N; ++k) sh[k * W + (threadIdx.x >> 6)] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) v[k] += sh[k * W + w];
+        }
     }
-    return v;
+}
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float *sh) {
+    float s[1] = {v};
+    row_sums<TPR>(s, sh);
+    return s[0];
 }
 
-// TPR threads hold a row in NP pieces of 16 bytes each
+// TPR threads hold a row in NP pieces of 16 bytes each.  fetch() brings them as
+// they lie in memory, of the row's end where a piece passes it, so that nothing
+// waits for them; take() gives one as floats, zeros behind the row.  Rows
+// shorter than a piece are finished in fetch() (`tiny`).
 template <typename T, int TPR, int NP> struct Rows {
     static constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR, V = VEC<T>;
+    int t, D;
+    bool tiny;
+    __device__ __forceinline__ Rows(int d) : t(threadIdx.x % TPR), D(d), tiny(d < V) {}
+    __device__ __forceinline__ int column(int p) const { return (p * TPR + t) * V; }
+    __device__ __forceinline__ void fetch(const T *row, u4 (&v)[NP]) const {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = column(p);
+            v[p] = tiny ? load(row, 0, c ? 0 : D).u : reinterpret_cast<const Un16<T> *>(row + min(c, D - V))->v;
+        }
+    }
+    __device__ __forceinline__ void take(u4 u, int p, float (&v)[V]) const {
+        const int n = D - column(p);
+        if (n < V && !tiny) u = n > 0 ? shift_down(u, (V - n) * 8 * (int)sizeof(T)) : u4{0, 0, 0, 0};
+        Piece<T> w;
+        w.u = u;
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = (float)w.e[q];
+    }
+    // gamma or beta of the thread's columns; `none` where there is none
+    __device__ __forceinline__ void params(const float *g, float none, float (&v)[NP][V]) const {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int c = column(p);
+            if (g && c + V <= D) {
+                Un16<float> w[V / 4];
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) w[q] = *reinterpret_cast<const Un16<float> *>(g + c + 4 * q);
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[p][q] = __uint_as_float(w[q / 4].v[q % 4]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[p][q] = g && c + q < D ? g[c + q] : none;
+            }
+        }
+    }
 };
 
+// The next row of a thread is on its way while it works on one.
 template <typename T, int TPR, int NP>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(Args a) {
     using L = Rows<T, TPR, NP>;
     constexpr int V = L::V;
     __shared__ float sh[16];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const L l(a.D);
+    const int slot = threadIdx.x / TPR;
     const float inv = 1.f / (float)a.D;
+    const T *X = reinterpret_cast<const T *>(a.x);
+    const long long stride = (long long)gridDim.x * L::ROWS;
+    long long r = (long long)blockIdx.x * L::ROWS + slot;
+    u4 next[NP];
+    l.fetch(X + min(r, a.rows - 1) * a.ldx, next);
     float g[NP][V], b[NP][V];
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const int c = (p * TPR + t) * V + q;
-            g[p][q] = a.gamma && c < a.D ? a.gamma[c] : 1.f;
-            b[p][q] = a.beta && c < a.D ? a.beta[c] : 0.f;
-        }
-    for (long long r = (long long)blockIdx.x * L::ROWS + slot; r - slot < a.rows; r += (long long)gridDim.x * L::ROWS) {
-        const bool live = r < a.rows;
-        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.ldx;
+    l.params(a.gamma, 1.f, g);
+    l.params(a.beta, 0.f, b);
+    for (; r - slot < a.rows; r += stride) {
         float v[NP][V], s = 0.f;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const int c = (p * TPR + t) * V;
-            const Piece<T> w = load(x + c, live ? a.D - c : 0);
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                v[p][q] = (float)w.e[q];
-                s += v[p][q];
-            }
-        }
-        const float mean = row_sum<TPR>(s, sh) * inv;
-        s = 0.f;
+        for (int p = 0; p < NP; ++p) l.take(next[p], p, v[p]);
+        l.fetch(X + min(r + stride, a.rows - 1) * a.ldx, next);
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int q = 0; q < V; ++q) {
-                v[p][q] = (p * TPR + t) * V + q < a.D ? v[p][q] - mean : 0.f;
-                s += v[p][q] * v[p][q];
-            }
+            for (int q = 0; q < V; ++q) s += v[p][q];
+        const float mean = row_sum<TPR>(s, sh) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[p][q] -= mean;
+            if (l.column(p) + V > a.D)  // nothing behind the row
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[p][q] = l.column(p) + q < a.D ? v[p][q] : 0.f;
+#pragma unroll
+            for (int q = 0; q < V; ++q) s += v[p][q] * v[p][q];
+        }
         const float rstd = 1.f / sqrtf(row_sum<TPR>(s, sh) * inv + a.eps);
-        if (!live) continue;
+        if (r >= a.rows) continue;
         T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            const int c = (p * TPR + t) * V;
             Piece<T> w;
 #pragma unroll
             for (int q = 0; q < V; ++q) w.e[q] = (T)(v[p][q] * rstd * g[p][q] + b[p][q]);
-            store(o + c, w, a.D - c);
+            store(o + l.column(p), w, a.D - l.column(p));
         }
-        if (t == 0) {
+        if (l.t == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
         }
@@ -139,57 +217,78 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(Args a) {
 }
 
 // dx, and each workgroup's share of dg and db: a thread keeps the sums of its
-// columns over all rows it takes; the row slots are added through LDS at the end.
+// columns over all rows it takes; the row slots are added through LDS at the
+// end.
 template <typename T, int TPR, int NP>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(Args a) {
     using L = Rows<T, TPR, NP>;
     constexpr int V = L::V;
-    __shared__ float sh[16];
+    // of 32 columns to a thread the registers hold the sums and one row: gamma
+    // is read again, and no second row is on its way
+    constexpr bool KEEP = NP * V < 32, AHEAD = NP * V < 32;
+    __shared__ float sh[32];
     __shared__ float cols[L::ROWS > 1 ? L::THREADS * NP * V : 1];
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+    const L l(a.D);
+    const int slot = threadIdx.x / TPR;
     const float inv = 1.f / (float)a.D;
-    float g[NP][V], dg[NP][V], db[NP][V];
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int q = 0; q < V; ++q) {
-            const int c = (p * TPR + t) * V + q;
-            g[p][q] = a.gamma && c < a.D ? a.gamma[c] : 1.f;
-            dg[p][q] = db[p][q] = 0.f;
-        }
-    for (long long r = (long long)blockIdx.x * L::ROWS + slot; r - slot < a.rows; r += (long long)gridDim.x * L::ROWS) {
+    const T *X = reinterpret_cast<const T *>(a.x), *DY = reinterpret_cast<const T *>(a.dy);
+    const long long stride = (long long)gridDim.x * L::ROWS;
+    long long r = (long long)blockIdx.x * L::ROWS + slot;
+    u4 nx[NP], ny[NP];
+    float nm = 0.f, nr = 0.f;
+    auto fetch = [&](long long i) {
+        const long long k = min(i, a.rows - 1);
+        l.fetch(X + k * a.ldx, nx);
+        l.fetch(DY + k * a.ldy, ny);
+        nm = a.mean[k];
+        nr = a.rstd[k];
+    };
+    if (AHEAD && a.rows > 0) fetch(r);
+    float g[NP][V], dg[NP][V] = {}, db[NP][V] = {};
+    if (KEEP) l.params(a.gamma, 1.f, g);
+    for (; r - slot < a.rows; r += stride) {
         const bool live = r < a.rows;
-        const T *x = reinterpret_cast<const T *>(a.x) + (live ? r : 0) * a.ldx;
-        const T *dy = reinterpret_cast<const T *>(a.dy) + (live ? r : 0) * a.ldy;
-        const float mean = live ? a.mean[r] : 0.f, rstd = live ? a.rstd[r] : 0.f;
-        float h[NP][V], d[NP][V], s1 = 0.f, s2 = 0.f;
+        if (!AHEAD) fetch(r);
+        // a row that is not there counts as zeros; behind a row dy is zero, so
+        // that what x - mean gives there reaches no sum
+        if (!live) {
+            nm = nr = 0.f;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) nx[p] = ny[p] = u4{0, 0, 0, 0};
+        }
+        const float mean = nm, rstd = nr;
+        float h[NP][V], d[NP][V], s[2] = {};
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            const int c = (p * TPR + t) * V;
-            const Piece<T> w = load(x + c, live ? a.D - c : 0), y = load(dy + c, live ? a.D - c : 0);
+            l.take(nx[p], p, h[p]);
+            l.take(ny[p], p, d[p]);
+        }
+        if (AHEAD) fetch(r + stride);
+        if (!KEEP) l.params(a.gamma, 1.f, g);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
             for (int q = 0; q < V; ++q) {
-                const float e = (float)y.e[q];
-                h[p][q] = live && c + q < a.D ? ((float)w.e[q] - mean) * rstd : 0.f;
+                h[p][q] = (h[p][q] - mean) * rstd;
+                const float e = d[p][q];
                 dg[p][q] += e * h[p][q];
                 db[p][q] += e;
                 d[p][q] = e * g[p][q];
-                s1 += d[p][q];
-                s2 += d[p][q] * h[p][q];
+                s[0] += d[p][q];
+                s[1] += d[p][q] * h[p][q];
             }
-        }
         if (!a.out) continue;
-        s1 = row_sum<TPR>(s1, sh) * inv;
-        s2 = row_sum<TPR>(s2, sh) * inv;
+        row_sums<TPR>(s, sh);
+        s[0] *= inv;
+        s[1] *= inv;
         if (!live) continue;
         T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-            const int c = (p * TPR + t) * V;
             Piece<T> w;
 #pragma unroll
-            for (int q = 0; q < V; ++q) w.e[q] = (T)(rstd * (d[p][q] - s1 - h[p][q] * s2));
-            store(o + c, w, a.D - c);
+            for (int q = 0; q < V; ++q) w.e[q] = (T)(rstd * (d[p][q] - s[0] - h[p][q] * s[1]));
+            store(o + l.column(p), w, a.D - l.column(p));
         }
     }
     if (!a.part) return;
@@ -201,7 +300,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(Args a)
 #pragma unroll
             for (int p = 0; p < NP; ++p)
 #pragma unroll
-                for (int q = 0; q < V; ++q) cols[slot * TPR * NP * V + (p * TPR + t) * V + q] = k ? db[p][q] : dg[p][q];
+                for (int q = 0; q < V; ++q) cols[slot * TPR * NP * V + l.column(p) + q] = k ? db[p][q] : dg[p][q];
             __syncthreads();
             for (int c = threadIdx.x; c < TPR * NP * V && c < a.D; c += L::THREADS) {
                 float v = 0.f;
@@ -214,7 +313,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(Args a)
             for (int p = 0; p < NP; ++p)
 #pragma unroll
                 for (int q = 0; q < V; ++q) {
-                    const int c = (p * TPR + t) * V + q;
+                    const int c = l.column(p) + q;
                     if (c < a.D) o[c] = k ? db[p][q] : dg[p][q];
                 }
         }
@@ -230,14 +329,14 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide(Args a
     T *o = reinterpret_cast<T *>(a.out) + r * a.ldo;
     float s = 0.f;
     for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        const Piece<T> w = load(x + c, (int)(a.D - c));
+        const Piece<T> w = load(x + c, (int)c, (int)(a.D - c));
 #pragma unroll
         for (int q = 0; q < V; ++q) s += (float)w.e[q];
     }
     const float mean = row_sum<1024>(s, sh) / (float)a.D;
     s = 0.f;
     for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        const Piece<T> w = load(x + c, (int)(a.D - c));
+        const Piece<T> w = load(x + c, (int)c, (int)(a.D - c));
 #pragma unroll
         for (int q = 0; q < V; ++q) {
             const float d = c + q < a.D ? (float)w.e[q] - mean : 0.f;
@@ -246,7 +345,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide(Args a
     }
     const float rstd = 1.f / sqrtf(row_sum<1024>(s, sh) / (float)a.D + a.eps);
     for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        Piece<T> w = load(x + c, (int)(a.D - c));
+        Piece<T> w = load(x + c, (int)c, (int)(a.D - c));
 #pragma unroll
         for (int q = 0; q < V; ++q)
             if (c + q < a.D)
@@ -268,7 +367,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide_backwa
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s1 = 0.f, s2 = 0.f;
     for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        const Piece<T> w = load(x + c, (int)(a.D - c)), y = load(dy + c, (int)(a.D - c));
+        const Piece<T> w = load(x + c, (int)c, (int)(a.D - c)), y = load(dy + c, (int)c, (int)(a.D - c));
 #pragma unroll
         for (int q = 0; q < V; ++q)
             if (c + q < a.D) {
@@ -280,7 +379,7 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide_backwa
     s1 = row_sum<1024>(s1, sh) / (float)a.D;
     s2 = row_sum<1024>(s2, sh) / (float)a.D;
     for (long long c = threadIdx.x * V; c < a.D; c += 1024 * V) {
-        const Piece<T> w = load(x + c, (int)(a.D - c)), y = load(dy + c, (int)(a.D - c));
+        const Piece<T> w = load(x + c, (int)c, (int)(a.D - c)), y = load(dy + c, (int)c, (int)(a.D - c));
         Piece<T> z = w;
 #pragma unroll
         for (int q = 0; q < V; ++q)
@@ -344,54 +443,85 @@ __global__ __launch_bounds__(1024) void k_norm_join(const float *part, int n, in
 }
 
 // ---- host ---------------------------------------------------------------
-// (threads per row, pieces per thread) for D elements: 0 = wider than any
+// The layout of rows of D elements: the first of these that holds their pieces
+// of 16 bytes, 0 for wider ones.  A thread's pieces stay in registers, forward
+// next to gamma and beta, backward next to gamma and the sums of dg and db, so
+// that backward has at most 256 registers' worth of threads to a row.
 static int layout(int D, int dtype) {
     const long long pieces = ((long long)D * (dtype == 0 ? 4 : 2) + 15) / 16;
-    const int cap[] = {16, 32, 64, 128, 256, 512, 1024, 2048};
-    for (int i = 0; i < 8; ++i)
+    const int cap[] = {16, 32, 64, 128, 192, 256, 512, 1024, 2048, 4096};
+    for (int i = 0; i < (dtype == 0 ? 10 : 9); ++i)
         if (pieces <= cap[i]) return i + 1;
     return 0;
 }
-static int rows_per_group(int lay) { return lay == 1 ? 16 : lay == 2 ? 8 : lay <= 5 ? 4 : 1; }
-// workgroups of the backward pass: two on each CU, each with a share of dg and db
+// workgroups of the backward pass, each with a share of dg and db
 static int backward_groups(long long rows, int D, int dtype) {
     const int lay = layout(D, dtype);
     if (!lay) return (int)std::min<long long>(64, std::max<long long>(1, rows / 16));
-    return (int)std::max<long long>(1, std::min<long long>(ceil_div(rows, rows_per_group(lay)), 512));
+    const int slots = lay == 1 ? 16 : lay == 2 ? 8 : lay <= (dtype == 0 ? 6 : 5) ? 4 : 1;  // rows at once
+    const int most = lay <= 3 || (dtype != 0 && lay == 6) ? 1024 : lay <= 7 ? 512 : 256;
+    // the shares (8 bytes a column, written and read) an eighth of the rows at most
+    const long long share = rows * (dtype == 0 ? 12 : 6) / 8 / 16;
+    return (int)std::max<long long>(1, std::min({ceil_div(rows, slots), (int64_t)most, (int64_t)std::max(share, 16ll)}));
 }
 
-template <typename T, int TPR, int NP> static void launch(const Args &a, bool back, int groups, hipStream_t s) {
+template <typename T, int TPR, int NP> static void launch_forward(const Args &a, hipStream_t s) {
     using L = Rows<T, TPR, NP>;
-    if (back) {
-        hipLaunchKernelGGL((k_norm_backward<T, TPR, NP>), dim3(groups), dim3(L::THREADS), 0, s, a);
-        return;
-    }
-    const unsigned grid = (unsigned)std::min<long long>(ceil_div(a.rows, L::ROWS), 4096);
+    // as many as a CU holds: each takes gamma and beta once (4096 workgroups read
+    // 32000 rows of 1024 in bf16 in 64 us, for the sake of their 8 KiB)
+    const unsigned grid = (unsigned)std::min<long long>(ceil_div(a.rows, L::ROWS), 256 * 2048 / L::THREADS);
     hipLaunchKernelGGL((k_norm<T, TPR, NP>), dim3(grid), dim3(L::THREADS), 0, s, a);
+}
+template <typename T, int TPR, int NP> static void launch_backward(const Args &a, int groups, hipStream_t s) {
+    hipLaunchKernelGGL((k_norm_backward<T, TPR, NP>), dim3(groups), dim3(Rows<T, TPR, NP>::THREADS), 0, s, a);
+}
+template <typename T> static void run_forward(const Args &a, int lay, hipStream_t s) {
+    switch (lay) {
+        case 1: return launch_forward<T, 16, 1>(a, s);
+        case 2: return launch_forward<T, 32, 1>(a, s);
+        case 3: return launch_forward<T, 64, 1>(a, s);
+        case 4: return launch_forward<T, 64, 2>(a, s);
+        case 5: return launch_forward<T, 64, 3>(a, s);
+        case 6: return launch_forward<T, 256, 1>(a, s);
+        case 7: return launch_forward<T, 256, 2>(a, s);
+        case 8: return launch_forward<T, 1024, 1>(a, s);
+        case 9: return launch_forward<T, 1024, 2>(a, s);
+    }
+    if constexpr (sizeof(T) == 4)
+        if (lay == 10) return launch_forward<T, 1024, 4>(a, s);
+    hipLaunchKernelGGL(k_norm_wide<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
+}
+template <typename T> static void run_backward(const Args &a, int lay, int groups, hipStream_t s) {
+    switch (lay) {
+        case 1: return launch_backward<T, 16, 1>(a, groups, s);
+        case 2: return launch_backward<T, 32, 1>(a, groups, s);
+        case 3: return launch_backward<T, 64, 1>(a, groups, s);
+        case 4: return launch_backward<T, 64, 2>(a, groups, s);
+        case 7: return launch_backward<T, 256, 2>(a, groups, s);
+        case 9: return launch_backward<T, 512, 4>(a, groups, s);
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (lay == 5 || lay == 6) return launch_backward<T, 64, 4>(a, groups, s);
+        if (lay == 8) return launch_backward<T, 256, 4>(a, groups, s);
+        if (lay == 10) return launch_backward<T, 512, 8>(a, groups, s);
+    } else {
+        if (lay == 5) return launch_backward<T, 64, 3>(a, groups, s);
+        if (lay == 6) return launch_backward<T, 256, 1>(a, groups, s);
+        if (lay == 8) return launch_backward<T, 512, 2>(a, groups, s);
+    }
+    // the sums first: dx may be written over dy
+    if (a.part)
+        hipLaunchKernelGGL(k_norm_wide_sums<T>, dim3((unsigned)ceil_div(a.D, 64), groups), dim3(256), 0, s, a);
+    if (a.out && a.rows)
+        hipLaunchKernelGGL(k_norm_wide_backward<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
 }
 template <typename T> static int run(const char *fn, const Args &a, int dtype, bool back, float *dg, float *db,
                                      hipStream_t s) {
     const int groups = backward_groups(a.rows, a.D, dtype), lay = layout(a.D, dtype);
-    switch (lay) {
-        case 1: launch<T, 16, 1>(a, back, groups, s); break;
-        case 2: launch<T, 32, 1>(a, back, groups, s); break;
-        case 3: launch<T, 64, 1>(a, back, groups, s); break;
-        case 4: launch<T, 64, 2>(a, back, groups, s); break;
-        case 5: launch<T, 64, 4>(a, back, groups, s); break;
-        case 6: launch<T, 256, 2>(a, back, groups, s); break;
-        case 7: launch<T, 256, 4>(a, back, groups, s); break;
-        case 8: launch<T, 1024, 2>(a, back, groups, s); break;
-        default:
-            if (!back) {
-                hipLaunchKernelGGL(k_norm_wide<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
-                break;
-            }
-            // the sums first: dx may be written over dy
-            if (a.part)
-                hipLaunchKernelGGL(k_norm_wide_sums<T>, dim3((unsigned)ceil_div(a.D, 64), groups), dim3(256), 0, s, a);
-            if (a.out && a.rows)
-                hipLaunchKernelGGL(k_norm_wide_backward<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
-    }
+    if (back)
+        run_backward<T>(a, lay, groups, s);
+    else
+        run_forward<T>(a, lay, s);
     MDX_CHECK_LAUNCH(fn);
     if (back && a.part) {
         hipLaunchKernelGGL(k_norm_join, dim3((unsigned)ceil_div(a.D, 16), 2), dim3(1024), 0, s, a.part, groups, a.D, dg,
