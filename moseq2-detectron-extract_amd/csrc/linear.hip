@@ -286,6 +286,22 @@ __device__ __forceinline__ void map_tile(unsigned id, unsigned ti, unsigned tj, 
     u = in / rows;
 }
 
+// The k-th longest of up to 64 groups (of equal ones the first), and how many
+// have more than `rows` rows: long reductions are started first.
+__device__ __forceinline__ int ranked_group(const Groups &g, int E, int k) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t mine = g.end - g.start;
+    int rank = 0;
+    for (int l = 0; l < E; ++l) {
+        const uint32_t n = __builtin_amdgcn_readlane(mine, l);
+        rank += n > mine || (n == mine && l < lane);
+    }
+    return __ffsll(__ballot(lane < E && rank == k)) - 1;
+}
+__device__ __forceinline__ int groups_above(const Groups &g, uint32_t rows) {
+    return __popcll(__ballot(g.end - g.start > rows));  // lanes without a group have none
+}
+
 // What a workgroup computes: rows i0 .. of i1, columns from j0, the reduction
 // r0 .. r1, and the offsets of its group and slice.
 struct Where {
@@ -325,26 +341,31 @@ template <int MODE> __device__ __forceinline__ bool place(const Args &g, int id,
         w.j0 = bj * u;
         return true;
     }
-    int e = 0, z = 0;
-    if (MODE == GROUP_RED || g.splits > 1) {
-        const int per = g.ti * g.tj;
-        w.grp = id / per;
-        id -= w.grp * per;
-        z = w.grp;
+    int z = 0;
+    if (MODE == GROUP_RED || g.splits > 1) {  // a group's slices follow each other, the longest group first
+        const int per = g.ti * g.tj, k = id / per;
+        id -= k * per;
+        z = MODE == GROUP_RED ? k % g.splits : k;
+        w.grp = z;
         if (MODE == GROUP_RED) {
-            z = w.grp / g.E;
-            e = w.grp - z * g.E;
+            int e = k / g.splits;
+            Span s;
+            if (g.E <= 64) {
+                const Groups all(g.counts, g.E, g.T, 1, 0, 0, 0);
+                e = ranked_group(all, g.E, e);
+                s = all.span(1ull << e, 0, 0);
+            } else {
+                s = find_group(g.counts, g.E, g.T, 1, e);
+            }
+            w.grp = z * g.E + e;
+            w.r0 = s.start;
+            w.r1 = s.end;
+            w.ooff = e * g.gstride;
         }
     }
     map_tile(id, g.ti, g.tj, t, u);
     w.i0 = (long long)bi * t;
     w.j0 = bj * u;
-    if (MODE == GROUP_RED) {
-        const Span s = find_group(g.counts, g.E, g.T, 1, e);
-        w.r0 = s.start;
-        w.r1 = s.end;
-        w.ooff = e * g.gstride;
-    }
     if (g.splits > 1) {  // this slice of the reduction, in whole steps
         const int steps = (int)((w.r1 - w.r0 + bk - 1) / bk), per = (steps + g.splits - 1) / g.splits;
         w.r0 = min(w.r1, w.r0 + (long long)z * per * bk);
@@ -1075,15 +1096,21 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_forward(Args g) {
     run_tile<T, false, false, MODE, KIND>(g, lds, blockIdx.x);
 }
 // dW's tiles and dx's in one launch: they need nothing of each other, and
-// either alone often leaves part of the CUs without a tile (dW has few, long
-// ones, which come first).
+// either alone often leaves part of the CUs without a tile.  Of dW's nw tiles
+// the `first` ones come before dx's, whose reduction is x.R: those that reduce
+// more (grouped: of the groups with more rows).
 template <typename T, bool GROUPED, int KIND>
-__global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int nw, Args x) {
+__global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int nw, int nx, int first, Args x) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    if ((int)blockIdx.x < nw)
-        run_tile<T, true, true, GROUPED ? GROUP_RED : DENSE, KIND>(w, lds, blockIdx.x);
-    else
-        run_tile<T, false, true, GROUPED ? GROUP_ROWS : DENSE, KIND>(x, lds, blockIdx.x - nw);
+    int id = blockIdx.x;
+    if (GROUPED && first < 0)
+        first = groups_above(Groups(w.counts, w.E, w.T, 1, 0, 0, 0), (uint32_t)x.R * w.splits) * w.splits * w.ti * w.tj;
+    if (id >= first && id < first + nx) {
+        run_tile<T, false, true, GROUPED ? GROUP_ROWS : DENSE, KIND>(x, lds, id - first);
+    } else {
+        if (id >= first) id -= nx;
+        run_tile<T, true, true, GROUPED ? GROUP_RED : DENSE, KIND>(w, lds, id);
+    }
 }
 
 // The slices' partial sums, added in their order (no atomics: the same result
@@ -1346,8 +1373,12 @@ template <typename T, bool GROUPED, int KIND> static int launch_backward(Args w,
         if (x.out)
             if (int rc = set_tiles(x, GROUPED ? GROUP_ROWS : DENSE, side, side, threads, nx)) return rc;
         MDX_REQUIRE((nw + nx) * threads < (1ll << 31), "mdx_linear_backward: too many output tiles");
+        // without both, or with more groups than a wave has lanes: dW's first
+        const int first = !w.out || !x.out ? (int)nw
+                          : GROUPED        ? w.E <= 64 ? -1 : (int)nw
+                                           : w.R > x.R * w.splits ? (int)nw : 0;
         hipLaunchKernelGGL((k_backward<T, GROUPED, KIND>), dim3((unsigned)(nw + nx)), dim3(threads), tile_lds<T>(KIND), s,
-                           w, (int)nw, x);
+                           w, (int)nw, (int)nx, first, x);
         MDX_CHECK_LAUNCH("mdx_linear_backward");
         return w.out && w.splits > 1 ? launch_join<T, GROUPED>(w, s) : MDX_OK;
     }
