@@ -1072,6 +1072,65 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
         });
 }
 
+// ---- the bias's gradient ---------------------------------------------------
+// k_act_backward's arguments
+struct ActArgs {
+    const void *dy, *z;
+    long long ldy, ldz;
+    void *dz;            // or null: sums only
+    long long lddz;
+    float *part;         // or null: dz only
+    const int *counts;   // or null: one group of T rows
+    int E, rows;
+    long long T;
+    int N, act;
+    int zero_tail;       // write zeros to dz behind the last group
+};
+
+// units of bias_join: 16 columns of a group; a workgroup of the products'
+// launch, which takes its share of LDS with it, has several
+constexpr int BIAS_UNITS = 4;
+__host__ __device__ inline int bias_units(const ActArgs &g) { return (g.N + 15) / 16 * (g.E > 1 ? g.E : 1); }
+
+// db[e][n] = the sums of group e's chunks, always added in the same order.  256
+// threads have 16 columns, 16 threads to each, so that a hundred chunks are a
+// few loads in flight per thread and no chain of waits.
+__device__ __forceinline__ void bias_join(const ActArgs &g, float *db, int block) {
+    __shared__ float sh[4][16];
+    if (threadIdx.x >= 256) return;  // a wave that has ended is at no barrier
+    const int per = (g.N + 15) / 16, e = block / per, l = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const int col = (block - e * per) * 16 + l;
+    long long first = 0, n = (g.T + g.rows - 1) / g.rows;
+    if (g.counts) {
+        const Span s = find_group(g.counts, g.E, g.T, g.rows, e);
+        first = s.tile0;
+        n = ((long long)s.end - s.start + g.rows - 1) / g.rows;
+    }
+    float v = 0.f;
+    if (col < g.N) {
+        const float *p = g.part + first * g.N + col;
+        for (long long k = w; k < n; k += 8 * 16) {
+            float t[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) t[q] = k + 16 * q < n ? p[(k + 16 * q) * g.N] : 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += t[q];
+        }
+    }
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    __syncthreads();  // the unit before this one has been read
+    if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][l] = v;
+    __syncthreads();
+    if (threadIdx.x < 16 && col < g.N) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v += sh[k][l];
+        db[(long long)e * g.N + col] = v;
+    }
+}
+__global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) { bias_join(g, db, blockIdx.x); }
+
 // ---- kernels ----------------------------------------------------------------
 enum Kind { LARGE, DMA128, DMA64, REG128, REG64 };
 constexpr int tile_side(int kind) { return kind == LARGE ? BIG : kind == DMA128 || kind == REG128 ? 128 : 64; }
@@ -1098,11 +1157,17 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_forward(Args g) {
 // dW's tiles and dx's in one launch: they need nothing of each other, and
 // either alone often leaves part of the CUs without a tile.  Of dW's nw tiles
 // the `first` ones come before dx's, whose reduction is x.R: those that reduce
-// more (grouped: of the groups with more rows).
+// more (grouped: of the groups with more rows).  The bias's blocks come last.
 template <typename T, bool GROUPED, int KIND>
-__global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int nw, int nx, int first, Args x) {
+__global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int nw, int nx, int first, Args x,
+                                                                    ActArgs sums, float *db) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int id = blockIdx.x;
+    if (id >= nw + nx) {
+        const int units = bias_units(sums), first = (id - nw - nx) * BIAS_UNITS;
+        for (int u = first; u < min(units, first + BIAS_UNITS); ++u) bias_join(sums, db, u);
+        return;
+    }
     if (GROUPED && first < 0)
         first = groups_above(Groups(w.counts, w.E, w.T, 1, 0, 0, 0), (uint32_t)x.R * w.splits) * w.splits * w.ti * w.tj;
     if (id >= first && id < first + nx) {
@@ -1138,18 +1203,6 @@ __global__ __launch_bounds__(256) void k_product_join(Args g) {
 // workgroup takes one chunk of `rows` rows of a group by 32 pieces of 16 bytes;
 // its sums go to part[chunk][N], and k_bias_join adds a group's chunks.  Bound
 // by HBM.
-struct ActArgs {
-    const void *dy, *z;
-    long long ldy, ldz;
-    void *dz;            // or null: sums only
-    long long lddz;
-    float *part;         // or null: dz only
-    const int *counts;   // or null: one group of T rows
-    int E, rows;
-    long long T;
-    int N, act;
-    int zero_tail;       // write zeros to dz behind the last group
-};
 template <typename T>
 __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
     constexpr int W = VEC<T>, AT = 2;  // rows of a thread at once
@@ -1197,41 +1250,6 @@ __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
         if (col < g.N) g.part[(long long)blockIdx.y * g.N + col] = v;
     }
 }
-// db[e][n] = the sums of group e's chunks, always added in the same order.  A
-// workgroup has 16 columns and 16 threads to each, so that a hundred chunks are
-// a few loads in flight per thread and no chain of waits.
-__global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) {
-    __shared__ float sh[4][16];
-    const int l = threadIdx.x & 15, w = threadIdx.x >> 4, col = blockIdx.x * 16 + l;
-    long long first = 0, n = (g.T + g.rows - 1) / g.rows;
-    if (g.counts) {
-        const Span s = find_group(g.counts, g.E, g.T, g.rows, blockIdx.y);
-        first = s.tile0;
-        n = (s.end - s.start + g.rows - 1) / g.rows;
-    }
-    float v = 0.f;
-    if (col < g.N) {
-        const float *p = g.part + first * g.N + col;
-        for (long long k = w; k < n; k += 8 * 16) {
-            float t[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) t[q] = k + 16 * q < n ? p[(k + 16 * q) * g.N] : 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v += t[q];
-        }
-    }
-    v += __shfl_xor(v, 16);
-    v += __shfl_xor(v, 32);
-    if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][l] = v;
-    __syncthreads();
-    if (threadIdx.x < 16 && col < g.N) {
-        v = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v += sh[k][l];
-        db[(long long)blockIdx.y * g.N + col] = v;
-    }
-}
-
 // ---- host ---------------------------------------------------------------
 // rows of a forward call that k_product_few takes (grouped: on average)
 constexpr int FEW = 32;
@@ -1281,30 +1299,31 @@ static Choice choose(const Load *loads, int n, int es, bool aligned, long long m
     for (int kind = aligned ? (es == 2 ? LARGE : DMA128) : REG128; kind <= (aligned ? DMA64 : REG64); ++kind) {
         const Cost c = cost_of(kind, es);
         const int side = tile_side(kind);
-        for (int splits = 1; splits <= 16; ++splits) {
-            double tiles[2], steps[2], all = 0, part = 0;
+        for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            long long tiles[2], steps[2], all = 0, part = 0;
             bool fits = true;
             for (int k = 0; k < n; ++k) {
                 const Load &l = loads[k];
                 const int s = l.split ? splits : 1;
-                steps[k] = std::max(1.0, std::ceil((double)ceil_div(l.R * es, 128) / s));
+                steps[k] = std::max<long long>(1, ceil_div(ceil_div(l.R * es, 128), s));
                 if (s > 1 && steps[k] < 4) fits = false;
-                tiles[k] = (double)ceil_div(l.I, side) * ceil_div(l.J, side) * l.groups * s;
+                tiles[k] = ceil_div(l.I, side) * ceil_div(l.J, side) * l.groups * s;
                 all += tiles[k];
-                if (s > 1) part += 4.0 * s * l.I * l.J * (l.red ? l.groups : 1);
+                if (s > 1) part += 4 * s * l.I * l.J * (l.red ? l.groups : 1);
             }
             if (!fits || part > most_part) break;
-            const double here = std::min((double)c.slots, std::max(1.0, std::ceil(all / CUS)));
+            const long long here = std::min<long long>(c.slots, std::max<long long>(1, ceil_div(all, CUS)));
             const double step = std::max(c.alone, here * c.shared);
             double work = 0, longest = 0;
             for (int k = 0; k < n; ++k) {
-                work += tiles[k] * (steps[k] * step + c.fixed);
-                longest = std::max(longest, steps[k] * step + c.fixed);
+                const double t = (double)steps[k] * step + c.fixed;
+                work += (double)tiles[k] * t;
+                longest = std::max(longest, t);
             }
-            const double rounds = std::max(1.0, std::ceil(work / (longest * CUS * here) - 0.02));
-            const double us = rounds * longest + (part > 0 ? 5.0 + part / 4e6 : 0.0);
+            const double rounds = std::max(1.0, std::ceil(work / (longest * (double)(CUS * here)) - 0.02));
+            const double us = rounds * longest + (part > 0 ? 5.0 + (double)part / 4e6 : 0.0);
             if (us < 0.98 * best.us) best = Choice{kind, splits, us};
-            if (!loads[0].split) break;
+            if (!loads[0].split || all >= 8ll * CUS * c.slots) break;  // enough tiles as it is
         }
     }
     return best;
@@ -1362,8 +1381,10 @@ template <typename T, int MODE, int KIND> static int launch_forward(Args g, hipS
         return g.splits > 1 ? launch_join<T, false>(g, s) : MDX_OK;
     }
 }
-// w, x: dW's and dx's product, their pointer out null where not needed
-template <typename T, bool GROUPED, int KIND> static int launch_backward(Args w, Args x, hipStream_t s) {
+// w, x: dW's and dx's product, their pointer out null where not needed; db: the
+// bias's gradient from the sums of `sums`, or null
+template <typename T, bool GROUPED, int KIND>
+static int launch_backward(Args w, Args x, const ActArgs &sums, float *db, hipStream_t s) {
     if constexpr (KIND == LARGE && sizeof(T) == 4) return MDX_EINVAL;
     else {
         long long nw = 0, nx = 0;
@@ -1372,13 +1393,14 @@ template <typename T, bool GROUPED, int KIND> static int launch_backward(Args w,
             if (int rc = set_tiles(w, GROUPED ? GROUP_RED : DENSE, side, side, threads, nw)) return rc;
         if (x.out)
             if (int rc = set_tiles(x, GROUPED ? GROUP_ROWS : DENSE, side, side, threads, nx)) return rc;
-        MDX_REQUIRE((nw + nx) * threads < (1ll << 31), "mdx_linear_backward: too many output tiles");
+        const long long nb = db ? ceil_div(bias_units(sums), BIAS_UNITS) : 0;
+        MDX_REQUIRE((nw + nx + nb) * threads < (1ll << 31), "mdx_linear_backward: too many output tiles");
         // without both, or with more groups than a wave has lanes: dW's first
         const int first = !w.out || !x.out ? (int)nw
                           : GROUPED        ? w.E <= 64 ? -1 : (int)nw
                                            : w.R > x.R * w.splits ? (int)nw : 0;
-        hipLaunchKernelGGL((k_backward<T, GROUPED, KIND>), dim3((unsigned)(nw + nx)), dim3(threads), tile_lds<T>(KIND), s,
-                           w, (int)nw, (int)nx, first, x);
+        hipLaunchKernelGGL((k_backward<T, GROUPED, KIND>), dim3((unsigned)(nw + nx + nb)), dim3(threads),
+                           tile_lds<T>(KIND), s, w, (int)nw, (int)nx, first, x, sums, db);
         MDX_CHECK_LAUNCH("mdx_linear_backward");
         return w.out && w.splits > 1 ? launch_join<T, GROUPED>(w, s) : MDX_OK;
     }
@@ -1502,8 +1524,9 @@ static long long backward_bytes(const Shape &p, bool need_x, bool need_w, bool n
     return n;
 }
 
-template <typename T, bool GROUPED> static int backward(const Shape &p, const Back &b, hipStream_t s) {
-    const int E = std::max(p.E, 1), es = sizeof(T);
+template <typename T, bool GROUPED>
+static int backward(const char *fn, const Shape &p, const Back &b, int64_t ws_bytes, hipStream_t s) {
+    const int es = sizeof(T);
     // dz as the products take it; its rows in the workspace lie N apart
     const bool kept = p.act != MDX_ACT_NONE;
     const void *dz = !kept ? b.grad : b.dres ? b.dres : b.ws;
@@ -1511,8 +1534,11 @@ template <typename T, bool GROUPED> static int backward(const Shape &p, const Ba
     const bool al = pieces(dz, lddz, 0, p.N, es) && pieces(b.x, b.ldx, 0, p.K, es) &&
                     pieces(b.w, b.ldw, (long long)p.N * b.ldw, p.K, es);
     const BackPlan q = plan_backward(p, b.dx, b.dw, b.db, b.dres, al);
+    const long long need = q.dz_bytes + q.part_bytes + q.dw_bytes;
+    MDX_REQUIRE(need == 0 || (b.ws && ws_bytes >= need), "%s: needs %lld bytes of workspace, got %lld", fn, need,
+                (long long)ws_bytes);
+    ActArgs a{};
     if (q.dz || b.db || b.dres) {
-        ActArgs a{};
         a.dy = b.grad; a.ldy = b.ldg;
         a.z = b.pre; a.ldz = b.ldp;
         a.dz = b.dres ? b.dres : q.dz ? b.ws : nullptr;
@@ -1525,10 +1551,6 @@ template <typename T, bool GROUPED> static int backward(const Shape &p, const Ba
         const dim3 grid((unsigned)ceil_div(p.N, 32 * VEC<T>), (unsigned)act_chunks(p.E, p.T, q.rows));
         hipLaunchKernelGGL(k_act_backward<T>, grid, dim3(256), 0, s, a);
         MDX_CHECK_LAUNCH("mdx_linear_backward");
-        if (b.db) {
-            hipLaunchKernelGGL(k_bias_join, dim3((unsigned)ceil_div(p.N, 16), E), dim3(256), 0, s, a, b.db);
-            MDX_CHECK_LAUNCH("mdx_linear_backward");
-        }
     }
     Args w{}, x{};
     w.splits = x.splits = 1;
@@ -1551,21 +1573,28 @@ template <typename T, bool GROUPED> static int backward(const Shape &p, const Ba
         x.gstride = (long long)p.N * b.ldw;
         x.zero_tail = b.zero_tail;
     }
-    if (!w.out && !x.out) return MDX_OK;
+    if (!w.out && !x.out) {
+        if (b.db) {
+            hipLaunchKernelGGL(k_bias_join, dim3((unsigned)bias_units(a)), dim3(256), 0, s, a, b.db);
+            MDX_CHECK_LAUNCH("mdx_linear_backward");
+        }
+        return MDX_OK;
+    }
     switch (q.products.kind) {
-        case LARGE: return launch_backward<T, GROUPED, LARGE>(w, x, s);
-        case DMA128: return launch_backward<T, GROUPED, DMA128>(w, x, s);
-        case DMA64: return launch_backward<T, GROUPED, DMA64>(w, x, s);
-        case REG128: return launch_backward<T, GROUPED, REG128>(w, x, s);
-        default: return launch_backward<T, GROUPED, REG64>(w, x, s);
+        case LARGE: return launch_backward<T, GROUPED, LARGE>(w, x, a, b.db, s);
+        case DMA128: return launch_backward<T, GROUPED, DMA128>(w, x, a, b.db, s);
+        case DMA64: return launch_backward<T, GROUPED, DMA64>(w, x, a, b.db, s);
+        case REG128: return launch_backward<T, GROUPED, REG128>(w, x, a, b.db, s);
+        default: return launch_backward<T, GROUPED, REG64>(w, x, a, b.db, s);
     }
 }
 
 template <typename T> static int forward_any(const Shape &p, const Args &g, int64_t ws_bytes, hipStream_t s) {
     return p.E ? forward<T, GROUP_ROWS>(p, g, ws_bytes, s) : forward<T, DENSE>(p, g, ws_bytes, s);
 }
-template <typename T> static int backward_any(const Shape &p, const Back &b, hipStream_t s) {
-    return p.E ? backward<T, true>(p, b, s) : backward<T, false>(p, b, s);
+template <typename T>
+static int backward_any(const char *fn, const Shape &p, const Back &b, int64_t ws_bytes, hipStream_t s) {
+    return p.E ? backward<T, true>(fn, p, b, ws_bytes, s) : backward<T, false>(fn, p, b, ws_bytes, s);
 }
 static int run_forward(const char *fn, const Shape &p, const Args &g, int64_t ws_bytes, hipStream_t s) {
     MDX_REQUIRE(g.a && g.b && g.out, "%s: null pointer", fn);
@@ -1589,13 +1618,10 @@ static int run_backward(const char *fn, const Shape &p, const Back &b, int64_t w
                     !bad_ld(b.pre, b.ldp, p.N) && !bad_ld(b.dx, b.lddx, p.K) && !bad_ld(b.dw, b.lddw, p.K) &&
                     !bad_ld(b.dres, b.lddr, p.N),
                 "%s: a row stride is below its row's length", fn);
-    const long long need = backward_bytes(p, b.dx, b.dw, b.db, b.dres);
-    MDX_REQUIRE(need == 0 || (b.ws && ws_bytes >= need), "%s: needs %lld bytes of workspace, got %lld", fn, need,
-                (long long)ws_bytes);
     switch (p.dtype) {
-        case 0: return backward_any<float>(p, b, s);
-        case 1: return backward_any<_Float16>(p, b, s);
-        default: return backward_any<__bf16>(p, b, s);
+        case 0: return backward_any<float>(fn, p, b, ws_bytes, s);
+        case 1: return backward_any<_Float16>(fn, p, b, ws_bytes, s);
+        default: return backward_any<__bf16>(fn, p, b, ws_bytes, s);
     }
 }
 

@@ -171,12 +171,9 @@ def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
-def _output(out: Optional[torch.Tensor], shape, like: torch.Tensor, reads, inplace=()):
-    """(tensor to return, its rows): a new one, or the caller's `out`, which
-    must not share memory with `reads`, nor in part with `inplace`."""
-    if out is None:
-        out = torch.empty(shape, dtype=like.dtype, device=like.device)
-        return out, out if len(shape) == 2 else out.view(-1, shape[-1])
+def _output(out: torch.Tensor, reads, inplace=()) -> torch.Tensor:
+    """The rows of the caller's `out`, which must not share memory with
+    `reads`, nor in part with `inplace`."""
     rows = _rows(out, copy=False)
     if rows is None:
         raise ValueError("out must have rows of unit stride at a constant distance")
@@ -186,7 +183,7 @@ def _output(out: Optional[torch.Tensor], shape, like: torch.Tensor, reads, inpla
     for r in inplace:
         if r is not None and not _same(rows, r) and _overlap(rows, r):
             raise ValueError("out shares part of its memory with an input")
-    return out, rows
+    return rows
 
 
 def _ld(rows: Optional[torch.Tensor]) -> int:
@@ -266,10 +263,13 @@ def _forward(x, counts, weight, bias, residual, activation, return_pre, out):
         w = weight.contiguous() if grouped else _rows(weight)
         b = bias.contiguous() if bias is not None else None
         r = _rows(residual) if residual is not None else None
-        reads = (xr, w.view(-1, K) if grouped else w, None if b is None else b.view(1, -1))
         fresh = out is None
-        out, o = _output(out, shape, x, reads, (r,))
-        pre = torch.empty(shape, dtype=x.dtype, device=x.device) if return_pre else None
+        if fresh:
+            out = x.new_empty(shape)
+            o = out if len(shape) == 2 else out.view(-1, N)
+        else:
+            o = _output(out, (xr, w.view(-1, K), None if b is None else b.view(1, -1)), (r,))
+        pre = x.new_empty(shape) if return_pre else None
         p = pre.view(-1, N) if return_pre else None
         M, dt = xr.shape[0], _DTYPES[x.dtype]
         if M:
@@ -332,13 +332,13 @@ def _backward(grad, x, counts, weight, pre, activation, need_x, need_weight, nee
         w = weight.contiguous() if grouped else _rows(weight)
         z = _rows(pre) if act else None
         M, dt = xr.shape[0], _DTYPES[x.dtype]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_weight else None
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = x.new_empty(weight.shape) if need_weight else None
         db = torch.empty((E, N) if grouped else (N,), dtype=torch.float32, device=dev) if need_bias else None
         # without an activation the residual's gradient is grad, but for the
         # rows that no group holds
         own = need_residual and (act or grouped)
-        dr = torch.empty(shape, dtype=x.dtype, device=dev) if own else None
+        dr = x.new_empty(shape) if own else None
         flags = (int(need_x), int(need_weight), int(need_bias), int(own))
         if need_x or need_weight or need_bias or own:
             dxr, drr = (None if t is None else t.view(-1, t.shape[-1]) for t in (dx, dr))
@@ -376,7 +376,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, return_stats: bo
     with _on(x.device):
         xr = _rows(x)
         w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-        out, o = _output(out, tuple(x.shape), x, [None if t is None else t.view(1, -1) for t in (w, b)], (xr,))
+        if out is None:
+            out = x.new_empty(x.shape)
+            o = out if x.dim() == 2 else out.view(-1, D)
+        else:
+            o = _output(out, [None if t is None else t.view(1, -1) for t in (w, b)], (xr,))
         mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if return_stats else None
                       for _ in range(2))
         if xr.shape[0]:
@@ -406,7 +410,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, need_x: bool = True
         m, r = mean.contiguous(), rstd.contiguous()
         w = weight.contiguous() if weight is not None else None
         n, dt = xr.shape[0], _DTYPES[x.dtype]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dx = x.new_empty(x.shape) if need_x else None
         dw, db = (torch.empty(D, dtype=torch.float32, device=dev) if need else None
                   for need in (need_weight, need_bias))
         if need_x or need_weight or need_bias:
