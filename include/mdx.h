@@ -560,8 +560,10 @@ int mdx_heatmaps_to_keypoints(const float *maps, const float *boxes, const int *
  * 1 = float16, 3 = bfloat16; products accumulate in float32, outputs are
  * rounded once.  bias, gamma, beta and their gradients are float32.  Matrices
  * are row-major; ld* is the distance between rows in elements, at least the
- * row's length, with any alignment.  An output must not overlap an input,
- * except where it is exactly that buffer and the call says so.  No entry
+ * row's length, with any alignment (rows of whole 16-byte pieces at 16-byte
+ * addresses take the faster kernels); a workspace is 16-byte aligned.  At most
+ * 2^31 - 65537 rows or columns.  An output must not overlap an input, except
+ * where it is exactly that buffer and the call says so.  No entry
  * allocates or synchronises: all can be captured into a graph, and calls on
  * several streams run side by side on workspaces of their own.
  * ------------------------------------------------------------------- */

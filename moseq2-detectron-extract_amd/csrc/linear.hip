@@ -555,7 +555,7 @@ template <typename T, bool TR, int SIDE> struct RegOperand {
     const T *row[N];  // TR 0: the piece's row; TR 1: the piece in its row of the next step
     const T *base;    // TR 1: a piece that can always be read
     long long step;
-    int at, end, r0, left;  // TR 0: the piece's first r, the reduction's end; TR 1: its row of the next step, the end
+    int at, end, left;  // TR 0: the piece's first r, the reduction's end; TR 1: its row of the next step, the end
     bool in[N], tiny;       // TR 0: the row exists; TR 1: (left: elements of the piece's row from its first on)
     __device__ __forceinline__ void init(const T *p, long long ld, long long i0, long long I, long long r0_, long long R) {
         const int t = threadIdx.x, pc = t % S::PPR;
@@ -630,17 +630,21 @@ __device__ __forceinline__ void dma_barrier() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
 }
-// 16 bytes a lane from base + off to 1 KiB of LDS at dst (wave-uniform)
+// 16 bytes a lane to 1 KiB of LDS at dst (wave-uniform), from src or from
+// base + off.  m0 holds the place in LDS, one wait state before its use.  The
+// scalar operands may come straight from a v_readfirstlane: a vector memory
+// instruction may read such a register only five wait states later, which the
+// compiler does not see to inside inline asm.
 __device__ __forceinline__ void dma16(const void *src, uint32_t dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(dst)),
                  "v"(src)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
                      __builtin_amdgcn_readfirstlane(dst)),
                  "v"(off), "s"(uniform((long long)(uintptr_t)base))
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // ---- the small tiles ------------------------------------------------------
@@ -1090,7 +1094,7 @@ struct ActArgs {
 // units of bias_join: 16 columns of a group; a workgroup of the products'
 // launch, which takes its share of LDS with it, has several
 constexpr int BIAS_UNITS = 4;
-__host__ __device__ inline int bias_units(const ActArgs &g) { return (g.N + 15) / 16 * (g.E > 1 ? g.E : 1); }
+__host__ __device__ inline int bias_units(const ActArgs &g) { return (g.N / 16 + (g.N % 16 != 0)) * (g.E > 1 ? g.E : 1); }
 
 // db[e][n] = the sums of group e's chunks, always added in the same order.  256
 // threads have 16 columns, 16 threads to each, so that a hundred chunks are a
@@ -1251,8 +1255,6 @@ __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
     }
 }
 // ---- host ---------------------------------------------------------------
-// rows of a forward call that k_product_few takes (grouped: on average)
-constexpr int FEW = 32;
 constexpr int CUS = 256;  // of an MI355X
 
 struct Shape {
@@ -1406,7 +1408,7 @@ static int launch_backward(Args w, Args x, const ActArgs &sums, float *db, hipSt
     }
 }
 
-// Few rows to a group: 16 or 32 of them in a tile; 32 columns where that still
+// Few rows to a group: 16 of them in a tile, or 32 (dense); 32 columns where that still
 // gives every CU a few workgroups, else 16 and slices of the reduction until
 // every CU has one; 4, 8 or 16 waves to a slice of it.
 struct Few {
@@ -1447,19 +1449,37 @@ static int check_shape(const char *fn, const Shape &p) {
 }
 static bool bad_ld(const void *p, long long ld, long long width) { return p && ld < width; }
 
-static bool few_rows(const Shape &p) { return ceil_div(p.T, std::max(p.E, 1)) <= FEW; }
+// Whether k_product_few takes a forward call.  It reads weights faster than the
+// tiles do, and multiplies slower.  Dense: up to 32 rows (bf16 4096 x 4096: 1 row
+// 8.0 us against 12.0, 32 rows 14.1 against 14.9; fp32 14.5 against 29, 25 against
+// 29).  Of fp32 groups up to 16 rows each on average (8 x 4096 x 1024: 8 rows 29
+// us against 42, 20 rows 43 against 43).  The tiles of 16-bit groups fill the CUs
+// between them, so there the few take over with the length of the reduction, a
+// row for each 16 steps of 128 bytes (8 x 4096 x 1024: 1 row 10.4 us against 10.7,
+// 4 rows 13.5 against 14.1, 8 rows 17.5 against 14.9; 8 x 1024 x 4096: 4 rows 17
+// against 22, 16 rows 28 against 22; 4 x 1024 x 12544: 8 rows 23 against 59, 16
+// rows 48 against 59), and for each 64 where they are unaligned (8 x 4096 x 1023:
+// 1 row 26 us against 19; 8 x 1023 x 4095: 1 row 39 against 45, 4 rows 48 against
+// 45).
+static bool few_rows(const Shape &p, bool aligned) {
+    if (!p.E) return p.T <= 32;
+    if (p.dtype == 0) return p.T <= 16ll * p.E;
+    const long long steps = ceil_div((long long)p.K * p.es(), 128);
+    return p.T <= 16ll * p.E && p.T * (aligned ? 16 : 64) <= steps * p.E;
+}
 template <typename T, int MODE> static int forward(const Shape &p, Args g, int64_t ws_bytes, hipStream_t s) {
     g.splits = 1;
     const int es = sizeof(T);
-    if (few_rows(p)) {
+    const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
+    if (few_rows(p, al)) {
         const Few f = few_plan(ceil_div(p.T, std::max(p.E, 1)), p.E, p.N, p.K, es);
         if (f.splits > 1 && g.part && ws_bytes >= part_bytes(f.splits, 0, p.T, p.N)) g.splits = f.splits;
-        if (f.mt == 1)
-            return f.nt == 1 ? launch_few<T, MODE, 1, 1>(g, f.waves, s) : launch_few<T, MODE, 1, 2>(g, f.waves, s);
-        return f.nt == 1 ? launch_few<T, MODE, 2, 1>(g, f.waves, s) : launch_few<T, MODE, 2, 2>(g, f.waves, s);
+        if constexpr (MODE == DENSE)
+            if (f.mt == 2)
+                return f.nt == 1 ? launch_few<T, MODE, 2, 1>(g, f.waves, s) : launch_few<T, MODE, 2, 2>(g, f.waves, s);
+        return f.nt == 1 ? launch_few<T, MODE, 1, 1>(g, f.waves, s) : launch_few<T, MODE, 1, 2>(g, f.waves, s);
     }
     const Load l = forward_load(p);
-    const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
     const Choice c = choose(&l, 1, es, al, g.part ? ws_bytes : 0);
     g.splits = c.splits;
     switch (c.kind) {
@@ -1473,7 +1493,7 @@ template <typename T, int MODE> static int forward(const Shape &p, Args g, int64
 // room for the split that either kind of kernel chooses, aligned operands or not
 static long long forward_bytes(const Shape &p) {
     if (p.E) return 0;
-    if (few_rows(p)) return part_bytes(few_plan(p.T, 0, p.N, p.K, p.es()).splits, 0, p.T, p.N);
+    if (few_rows(p, true)) return part_bytes(few_plan(p.T, 0, p.N, p.K, p.es()).splits, 0, p.T, p.N);
     const Load l = forward_load(p);
     long long n = 0;
     for (int al = 0; al < 2; ++al)
@@ -1533,8 +1553,10 @@ static int backward(const char *fn, const Shape &p, const Back &b, int64_t ws_by
     const long long lddz = !kept ? b.ldg : b.dres ? b.lddr : p.N;
     const bool al = pieces(dz, lddz, 0, p.N, es) && pieces(b.x, b.ldx, 0, p.K, es) &&
                     pieces(b.w, b.ldw, (long long)p.N * b.ldw, p.K, es);
+    MDX_REQUIRE(!b.db || ceil_div(p.N, 16) * std::max(p.E, 1) < (1 << 23), "%s: too many columns of bias", fn);
     const BackPlan q = plan_backward(p, b.dx, b.dw, b.db, b.dres, al);
     const long long need = q.dz_bytes + q.part_bytes + q.dw_bytes;
+    MDX_REQUIRE(reinterpret_cast<uintptr_t>(b.ws) % 16 == 0, "%s: the workspace must be 16-byte aligned", fn);
     MDX_REQUIRE(need == 0 || (b.ws && ws_bytes >= need), "%s: needs %lld bytes of workspace, got %lld", fn, need,
                 (long long)ws_bytes);
     ActArgs a{};
@@ -1598,6 +1620,7 @@ static int backward_any(const char *fn, const Shape &p, const Back &b, int64_t w
 }
 static int run_forward(const char *fn, const Shape &p, const Args &g, int64_t ws_bytes, hipStream_t s) {
     MDX_REQUIRE(g.a && g.b && g.out, "%s: null pointer", fn);
+    MDX_REQUIRE(reinterpret_cast<uintptr_t>(g.part) % 16 == 0, "%s: the workspace must be 16-byte aligned", fn);
     MDX_REQUIRE(!bad_ld(g.a, g.lda, p.K) && !bad_ld(g.b, g.ldb, p.K) && !bad_ld(g.res, g.ldr, p.N) &&
                     !bad_ld(g.pre, g.ldp, p.N) && !bad_ld(g.out, g.ldo, p.N),
                 "%s: a row stride is below its row's length", fn);

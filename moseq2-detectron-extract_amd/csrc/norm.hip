@@ -580,6 +580,8 @@ extern "C" int mdx_layer_norm_backward(const void *grad, int64_t ldg, const void
     MDX_REQUIRE(ldg >= D && ldx >= D && (!dx || lddx >= D),
                 "mdx_layer_norm_backward: a row stride is below its row's length");
     const int64_t need = dgamma || dbeta ? mdx_layer_norm_backward_workspace_bytes(rows, D, dtype) : 0;
+    MDX_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+                "mdx_layer_norm_backward: the workspace must be 16-byte aligned");
     MDX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                 "mdx_layer_norm_backward: needs %lld bytes of workspace, got %lld", (long long)need,
                 (long long)workspace_bytes);

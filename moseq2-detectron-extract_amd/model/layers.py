@@ -232,6 +232,8 @@ def grouped_linear(x, counts, weight, bias=None, residual=None, activation=None,
     _check_input("x", x, 2)
     if x.dim() != 2:
         raise ValueError("x must be (T, K)")
+    if counts is None:
+        raise TypeError("counts must be a tensor")
     return _forward(x, counts, weight, bias, residual, activation, return_pre, out)
 
 
@@ -307,6 +309,8 @@ def grouped_linear_backward(grad, x, counts, weight, pre=None, activation=None, 
     _check_input("x", x, 2)
     if x.dim() != 2:
         raise ValueError("x must be (T, K)")
+    if counts is None:
+        raise TypeError("counts must be a tensor")
     return _backward(grad, x, counts, weight, pre, activation, need_x, need_weight, need_bias, need_residual)
 
 

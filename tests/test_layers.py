@@ -199,3 +199,34 @@ def test_workspace_sizes(mdx):
     assert call("mdx_linear_backward_workspace_bytes", 100, 30, 50, 1, 3, 1, 0, 0, 1) == 0  # dz goes to dres
     assert call("mdx_grouped_linear_backward_workspace_bytes", 0, 100, 30, 50, 1, 3, 1, 1, 1, 0) == 0
     assert call("mdx_layer_norm_backward_workspace_bytes", 100, 30, 3) >= 2 * 30 * 4
+
+
+def test_counts_are_needed(L):
+    """Without counts a grouped call is refused, a weight of two axes or not."""
+    x, dy = z(4, 8), z(4, 3)
+    for w in (z(3, 8), z(2, 3, 8)):
+        with pytest.raises(TypeError, match="counts"):
+            L.grouped_linear(x, None, w)
+        with pytest.raises(TypeError, match="counts"):
+            L.grouped_linear_backward(dy, x, None, w)
+
+
+def test_c_entries_refuse_unaligned_workspaces(mdx):
+    """Workspaces hold pieces of 16 bytes."""
+    p, odd, nul = ctypes.c_void_p(64), ctypes.c_void_p(72), None
+    calls = [("mdx_linear", (p, 8, p, 8, nul, nul, 0, 4, 3, 8, 0, 3, nul, 0, p, 3, odd, 1 << 20, nul)),
+             ("mdx_linear_backward", (p, 3, p, 8, p, 8, nul, 0, 4, 3, 8, 0, 3, p, 8, nul, 8, p, nul, 0, odd, 1 << 20, nul)),
+             ("mdx_grouped_linear_backward", (p, 3, p, 8, p, nul, 0, p, 2, 4, 3, 8, 0, 3, p, 8, nul, p, nul, 0, 1, odd,
+                                              1 << 20, nul)),
+             ("mdx_layer_norm_backward", (p, 8, p, 8, p, p, nul, 4, 8, 1, p, 8, p, nul, odd, 1 << 20, nul))]
+    for name, args in calls:
+        rc, text = _refused(name, *args)
+        assert rc == -1 and "16-byte aligned" in text, (name, rc, text)
+
+
+def test_c_entry_refuses_too_many_bias_columns(mdx):
+    """More columns of bias over all groups than a launch has threads for."""
+    p, nul = ctypes.c_void_p(64), None
+    rc, text = _refused("mdx_grouped_linear_backward", p, 1 << 20, p, 1, p, nul, 0, p, 4096, 4, 1 << 20, 1, 0, 3, nul, 1,
+                        nul, p, nul, 0, 1, p, 1 << 50, nul)
+    assert rc == -1 and "columns of bias" in text, (rc, text)

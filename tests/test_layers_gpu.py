@@ -736,3 +736,27 @@ def test_many_groups(L, E):
         check_forward(y[s:t], None, x[s:t], w[e], b[e], None, "silu", dt)
         check_backward(L_grads(got, e, s, t), dy[s:t], x[s:t], w[e], z[s:t], "silu", dt)
     assert (y[end:] == 0).all() and (got.x[end:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("E,per,N,K", [(4, 1, 40, 1024), (4, 4, 72, 4096), (3, 12, 33, 12544), (3, 13, 40, 12544),
+                                       (5, 1, 24, 8191), (8, 16, 264, 520), (8, 17, 264, 520), (70, 1, 48, 2048)])
+def test_grouped_few_rows(L, dt, E, per, N, K):
+    """Few rows to a group, long reductions and short ones, on both sides of
+    where another kernel takes over; one group holds most rows, one none."""
+    g = gen(E + per + N + K)
+    T = E * per
+    counts = [0] * E
+    counts[E // 2] = T - T // 4 - 1
+    for k in range(T // 4):
+        counts[k * 5 % E if k * 5 % E != 1 else 0] += 1
+    x, w, b, z, dy = grouped_inputs(T, E, N, K, dt, E + per)
+    r = normal(g, T, N, dtype=dt)
+    act = ACTS[(E + per) % 5]
+    cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    y, pre = L.grouped_linear(strided(x, 8), cd, w.cuda(), b.cuda(), r.cuda(), act, return_pre=True)
+    y, pre = y.cpu(), pre.cpu()
+    sp, end = spans(counts, T)
+    for e, (s, t) in enumerate(sp):
+        check_forward(y[s:t], pre[s:t], x[s:t], w[e], b[e], r[s:t], act, dt)
+    assert (y[end:] == 0).all() and (pre[end:] == 0).all()
