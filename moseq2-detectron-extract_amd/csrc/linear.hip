@@ -91,23 +91,25 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T *p, int
 // On the hardware's exp2 and reciprocal (1 ulp each): with the library's erff,
 // tanhf and division the epilogue of a 256 x 256 tile took longer than its
 // product of 1024 terms.
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-// 1 / (1 + exp(-u))
-__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-u)); }
+constexpr float LOG2E = 1.44269504088896341f;
+// 1 / (1 + exp2(u))
+__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u)); }
 // the normal distribution at z: *p its probability (1 + erf(z / sqrt 2)) / 2 by
 // formula 7.1.26 of Abramowitz and Stegun (erf to 1.5e-7), returned
 // exp(-z^2 / 2), which that formula needs and the density is made of
 __device__ __forceinline__ float normal_cdf(float z, float *p) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-    const float e = fast_exp(-x * x);
-    const float c =
-        0.5f * e * t *
-        (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.70710678118654752f) * fabsf(z));
+    const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E));
+    const float c = e * t * (0.5f * 0.254829592f + t * (0.5f * -0.284496736f + t * (0.5f * 1.421413741f +
+                    t * (0.5f * -1.453152027f + t * (0.5f * 1.061405429f)))));
     *p = z < 0.f ? c : 1.f - c;
     return e;
 }
-// the tanh form: (1 + tanh v) / 2 = logistic(2 v), 2 v = C (z + A z^3)
+// the tanh form: (1 + tanh v) / 2 = 1 / (1 + exp(-2 v)), 2 v = C (z + A z^3)
 constexpr float TANH_C = 1.59576912160573071f, TANH_A = 0.044715f;
+__device__ __forceinline__ float tanh_gate(float z) {
+    return logistic(z * (-TANH_C * LOG2E + (-TANH_C * TANH_A * LOG2E) * (z * z)));
+}
 
 __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
@@ -117,8 +119,8 @@ __device__ __forceinline__ float act_value(float z, int act) {
             normal_cdf(z, &p);
             return z * p;
         }
-        case MDX_ACT_GELU_TANH: return z * logistic(TANH_C * (z + TANH_A * z * z * z));
-        case MDX_ACT_SILU: return z * logistic(z);
+        case MDX_ACT_GELU_TANH: return z * tanh_gate(z);
+        case MDX_ACT_SILU: return z * logistic(-LOG2E * z);
         default: return z;
     }
 }
@@ -130,11 +132,11 @@ __device__ __forceinline__ float act_slope(float z, int act) {
             return p + z * e * 0.39894228040143268f;
         }
         case MDX_ACT_GELU_TANH: {
-            const float s = logistic(TANH_C * (z + TANH_A * z * z * z));
+            const float s = tanh_gate(z);
             return s + z * s * (1.f - s) * TANH_C * (1.f + 3.f * TANH_A * z * z);
         }
         case MDX_ACT_SILU: {
-            const float s = logistic(z);
+            const float s = logistic(-LOG2E * z);
             return s * (1.f + z * (1.f - s));
         }
         default: return 1.f;
@@ -374,10 +376,16 @@ template <int MODE> __device__ __forceinline__ bool place(const Args &g, int id,
     return true;
 }
 
+// a row: a part that is the same in all lanes, and the lane's
+struct Row {
+    long long u;
+    int l;
+    __device__ __forceinline__ long long at(long long ld) const { return u * ld + l * ld; }
+};
 // 16 bytes of a row of outputs from their sums v: bias b (zeros if there is
 // none), residual, activation and the stores
 template <typename T>
-__device__ __forceinline__ void finish(const Args &g, long long ooff, long long i, int j, float (&v)[VEC<T>],
+__device__ __forceinline__ void finish(const Args &g, long long ooff, Row i, int j, float (&v)[VEC<T>],
                                        const float (&b)[VEC<T>], u4 res) {
     constexpr int N = VEC<T>;
     const int n = g.J - j;
@@ -389,34 +397,37 @@ __device__ __forceinline__ void finish(const Args &g, long long ooff, long long 
     if (g.res)
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] += (float)r.e[q];
-    if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i * g.ldp + j, n, v);
+    if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i.at(g.ldp) + j, n, v);
     apply_act(v, g.act);
-    store_row<T, N>(reinterpret_cast<T *>(g.out) + ooff + i * g.ldo + j, n, v);
+    store_row<T, N>(reinterpret_cast<T *>(g.out) + ooff + i.at(g.ldo) + j, n, v);
 }
-template <typename T> __device__ __forceinline__ u4 load_residual(const Args &g, long long i, int j) {
-    return g.res ? load_piece(reinterpret_cast<const T *>(g.res) + i * g.ldr + j, j, g.J - j) : u4{0, 0, 0, 0};
+template <typename T> __device__ __forceinline__ u4 load_residual(const Args &g, Row i, int j) {
+    return g.res ? load_piece(reinterpret_cast<const T *>(g.res) + i.at(g.ldr) + j, j, g.J - j) : u4{0, 0, 0, 0};
 }
 // where the sums go: a slice's partial sums, zeros behind the last group, or
 // the finished outputs
 template <typename T>
-__device__ __forceinline__ void store_outputs(const Args &g, const Where &w, long long row, int col,
+__device__ __forceinline__ void store_outputs(const Args &g, const Where &w, Row row, int col,
                                               float (&v)[VEC<T>], const float (&b)[VEC<T>], u4 res) {
     constexpr int N = VEC<T>;
     const int n = g.J - col;
     if (g.splits > 1) {
-        store_row<float, N>(g.part + (w.grp * g.I + row) * g.J + col, n, v);
+        store_row<float, N>(g.part + w.grp * g.I * g.J + row.at(g.J) + col, n, v);
     } else if (w.tail) {
-        store_row<T, N>(reinterpret_cast<T *>(g.out) + row * g.ldo + col, n, v);
-        if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + row * g.ldp + col, n, v);
+        store_row<T, N>(reinterpret_cast<T *>(g.out) + row.at(g.ldo) + col, n, v);
+        if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + row.at(g.ldp) + col, n, v);
     } else {
         finish<T>(g, w.ooff, row, col, v, b, res);
     }
 }
 // A wave's sums, P blocks of 16 rows by Q columns (64 or 32) from column col0
-// on: block p, whose first row is row(p), is put by put(p, e) into the wave's
-// own epi_bytes(Q) of LDS e and from there finished, 16 bytes of a row to a
-// lane, so that a row's lanes store whole lines.  A lane's column is the same
-// in all blocks: its bias is loaded once, and the residual a block ahead.
+// on, AT of them at a time: blocks p .., whose first rows are row(p) .., are put
+// by put(p, e) into the wave's own epi_bytes(Q, AT) of LDS e and from there
+// finished, 16 bytes of a row to a lane, so that a row's lanes store whole
+// lines.  A lane's column is the same in all blocks: its bias is loaded once,
+// and the residual AT blocks ahead.  Two blocks at a time hide the way through
+// LDS (1000 x 1024 x 1024 bf16 GELU in 64-wide tiles 9.6 -> 8.9 us); beside the
+// 128 sums of a lane in the 256-wide tile there is room for one.
 // put_block is a 16 x 16 tile's part: lane (row l & 15, columns 4 (l >> 4)..);
 // slots of 16 bytes are XOR-swizzled by row against bank conflicts.
 template <int N, int K = 0, typename F> __device__ __forceinline__ void static_for(F f) {
@@ -425,48 +436,53 @@ template <int N, int K = 0, typename F> __device__ __forceinline__ void static_f
         static_for<N, K + 1>(f);
     }
 }
-constexpr int epi_bytes(int q) { return 16 * q * 4; }
+constexpr int epi_bytes(int q, int at) { return at * 16 * q * 4; }
 template <int Q> __device__ __forceinline__ void put_block(float *e, int j, f4 v) {
     const int lane = threadIdx.x & 63, r = lane & 15, slot = (4 * j + (lane >> 4)) ^ (r & (Q / 4 - 1));
     *reinterpret_cast<f4 *>(e + r * Q + 4 * slot) = v;
 }
-template <typename T, int Q, int P, typename R, typename F>
+template <typename T, int Q, int P, int AT, typename R, typename F>
 __device__ __forceinline__ void epilogue(const Args &g, const Where &w, char *lds, int col0, R row, F put) {
     constexpr int N = VEC<T>, PER = Q / N, K = 16 * PER / 64;  // PER lanes to a row, K pieces to a lane
-    const int lane = threadIdx.x & 63, c = lane % PER * N, col = col0 + c;
+    const int lane = threadIdx.x & 63, c = lane % PER * N, col = col0 + c, lr = lane / PER;
     float *e = reinterpret_cast<float *>(lds);
     const bool in = col < g.J, plain = g.splits == 1 && !w.tail;
     float b[N] = {};
     if (g.bias && plain) load_row<float, N>(g.bias + w.biasoff + col, col, in ? g.J - col : 0, b);
-    u4 next[K];
-    auto prefetch = [&](int p) {
+    auto each = [&](auto f) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const long long i = row(p) + (64 * k + lane) / PER;
-            next[k] = plain && in && i < w.i1 ? load_residual<T>(g, i, col) : u4{0, 0, 0, 0};
-        }
+        for (int h = 0; h < AT; ++h)
+#pragma unroll
+            for (int k = 0; k < K; ++k) f(h, k);
+    };
+    u4 next[AT][K];
+    auto prefetch = [&](int p) {
+        each([&](int h, int k) {
+            const Row i{row(p + h) + 64 / PER * k, lr};
+            next[h][k] = plain && in && i.u + lr < w.i1 ? load_residual<T>(g, i, col) : u4{0, 0, 0, 0};
+        });
     };
     prefetch(0);
 #pragma unroll 1
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < P; p += AT) {
         put(p, e);
-        u4 res[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) res[k] = next[k];
-        if (p + 1 < P) prefetch(p + 1);
+        u4 res[AT][K];
+        each([&](int h, int k) { res[h][k] = next[h][k]; });
+        if (p + AT < P) prefetch(p + AT);
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        float v[AT][K][N];
+        each([&](int h, int k) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int r = (64 * k + lane) / PER;
-            const long long i = row(p) + r;
-            if (i >= w.i1 || !in) continue;
-            float v[N];
-#pragma unroll
-            for (int q = 0; q < N / 4; ++q)
-                *reinterpret_cast<f4 *>(v + 4 * q) =
-                    *reinterpret_cast<const f4 *>(e + r * Q + 4 * ((c / 4 + q) ^ (r & (Q / 4 - 1))));
-            store_outputs<T>(g, w, i, col, v, b, res[k]);
-        }
+            for (int q = 0; q < N / 4; ++q) {
+                const int r = 64 / PER * k + lr;
+                *reinterpret_cast<f4 *>(v[h][k] + 4 * q) = *reinterpret_cast<const f4 *>(
+                    e + (16 * h + r) * Q + 4 * ((c / 4 + q) ^ (r & (Q / 4 - 1))));
+            }
+        });
+        each([&](int h, int k) {
+            const Row i{row(p + h) + 64 / PER * k, lr};
+            if (i.u + lr < w.i1 && in) store_outputs<T>(g, w, i, col, v[h][k], b, res[h][k]);
+        });
         __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     }
 }
@@ -700,7 +716,7 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
     using SB = Stage<T, TB, SIDE>;
     constexpr int Q = SIDE / 2, N = Q / 16;  // a wave's quarter, its MFMA tiles each way
     constexpr int STEP = SA::BYTES + SB::BYTES, NB = BUFS<T, SIDE, DMA>;
-    static_assert(4 * epi_bytes(Q) <= 2 * STEP, "the epilogue takes the operands' LDS");
+    static_assert(4 * epi_bytes(Q, 2) <= 2 * STEP, "the epilogue takes the operands' LDS");
     Where w;
     if (!place<MODE>(g, id, SIDE, SIDE, SA::BK, w)) return;
     const T *A = reinterpret_cast<const T *>(g.a), *B = reinterpret_cast<const T *>(g.b) + w.boff;
@@ -785,12 +801,13 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
             }
     }
     __syncthreads();  // the operands' buffers become the epilogue's
-    epilogue<T, Q, N>(
-        g, w, lds + wid * epi_bytes(Q), w.j0 + wj, [&](int p) { return w.i0 + wi + 16 * p; },
+    epilogue<T, Q, N, 2>(
+        g, w, lds + wid * epi_bytes(Q, 2), w.j0 + wj, [&](int p) { return w.i0 + wi + 16 * p; },
         [&](int p, float *e) {
-            static_for<N>([&](auto i) {
-                if (p == i) {
-                    static_for<N>([&](auto j) { put_block<Q>(e, j, acc[i][j]); });
+            static_for<N / 2>([&](auto i) {
+                if (p == 2 * i) {
+                    static_for<N>([&](auto j) { put_block<Q>(e, j, acc[2 * i][j]); });
+                    static_for<N>([&](auto j) { put_block<Q>(e + 16 * Q, j, acc[2 * i + 1][j]); });
                     asm volatile("; block %0" ::"n"(i.value));  // the branches stay apart: merged, they would
                 }                                               // index the accumulators, in memory
             });
@@ -871,7 +888,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
     for (int t = threadIdx.x; t < ROWS * COLS / N; t += 64 * WAVES) {
         const int r = t / (COLS / N), c = t % (COLS / N) * N;
         if (w.i0 + r >= w.i1 || w.j0 + c >= g.J) continue;
-        const u4 res = g.splits == 1 && !w.tail ? load_residual<T>(g, w.i0 + r, w.j0 + c) : u4{0, 0, 0, 0};
+        const u4 res = g.splits == 1 && !w.tail ? load_residual<T>(g, Row{w.i0, r}, w.j0 + c) : u4{0, 0, 0, 0};
         float v[N] = {}, b[N] = {};
         if (g.bias && g.splits == 1 && !w.tail)
             load_row<float, N>(g.bias + w.biasoff + w.j0 + c, w.j0 + c, g.J - w.j0 - c, b);
@@ -879,7 +896,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
         for (int k = 0; k < WAVES; ++k)
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] += red[k][r][c + e];
-        store_outputs<T>(g, w, w.i0 + r, w.j0 + c, v, b, res);
+        store_outputs<T>(g, w, Row{w.i0, r}, w.j0 + c, v, b, res);
     }
 }
 
@@ -1063,8 +1080,8 @@ __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
         tile(c2, c1, KT - 1, fy, fx);
         if (grp == 0) dma_barrier();  // every wave crosses as many, and has read all of this tile
     }
-    epilogue<T, 64, 8>(
-        g, w, lds + wid * epi_bytes(64), w.j0 + 64 * wn,
+    epilogue<T, 64, 8, 1>(
+        g, w, lds + wid * epi_bytes(64, 1), w.j0 + 64 * wn,
         [&](int p) { return w.i0 + 128 * (p >> 2) + 64 * grp + 16 * (p & 3); },
         [&](int p, float *e) {
             static_for<8>([&](auto k) {
@@ -1200,7 +1217,7 @@ __global__ __launch_bounds__(256) void k_product_join(Args g) {
     }
     float b[N] = {};
     if (g.bias) load_row<float, N>(g.bias + col, col, g.J - col, b);
-    finish<T>(g, blockIdx.y * g.gstride, row, col, v, b, load_residual<T>(g, row, col));
+    finish<T>(g, blockIdx.y * g.gstride, Row{row, 0}, col, v, b, load_residual<T>(g, Row{row, 0}, col));
 }
 
 // dz = dy act'(z) in T, and the column sums of dz before that rounding.  A
