@@ -9,7 +9,11 @@
 //   forward  i = row, j = n, r = k   x 0, W 0
 //   dx       i = row, j = k, r = n   dz 0, W 1
 //   dW       i = n,   j = k, r = row dz 1, x 1
-// so no operand is ever transposed in memory.
+// so no operand is ever transposed in memory.  Sums are float32 in the matrix
+// instructions; each output is rounded once.  dz is rounded to the operands'
+// type before the two products, since the matrix instructions take nothing
+// wider: a term is off by half a step of that type at most (bf16 gradients are
+// off by 0.0023 of their size on the whole, where rounded outputs alone give 0.0017).
 #include "common.h"
 
 #include <algorithm>
@@ -673,6 +677,12 @@ __device__ __forceinline__ void dma16s(const void *base, uint32_t off, uint32_t 
 // memory's latency at each step; one barrier a step, behind which step s has
 // landed everywhere and step s - 1 has been read, so that its buffer is free.
 // Otherwise: any alignment and sizes, through registers, two or three steps ahead.
+// 64-wide tiles are for products with too few tiles for the CUs: what bounds
+// them is a step's latency (DMA 0.28 us a step of 64 in bf16, through registers
+// 0.6), and they reach 235 TFLOP/s at 1000 x 1024 x 1024 bf16 (9.1 us) and 510 at
+// 1000 x 1024 x 12544 in two slices (50 us).  In float32 the matrix instructions
+// bound the 128-wide tile: 1000 x 1024 x 12544 in eight slices takes 208 us, of
+// which the join 7.4 (124 TFLOP/s of a peak of 157).
 template <typename T, int SIDE, bool DMA> constexpr int BUFS = !DMA || (sizeof(T) == 4 && SIDE == 128) ? 2 : 4;
 
 // a lane's part in staging one operand by DMA: instruction d of wave w brings
@@ -821,7 +831,9 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
 // every row at a time (lane: row l & 15, two pieces at 32 (l >> 4) bytes), four
 // such chunks in flight, straight from memory into the MFMAs; the waves' sums
 // meet in LDS.  Rows and columns beyond the end are clamped: their products are
-// not stored.
+// not stored.  Bound by the weight's way from memory, in small layers by the
+// chain of launch, load and join: bf16 1 x 4096 x 4096 8.1 us (4.2 TB/s), 16 x 1024
+// x 12544 in slices 12.1 (2.1 TB/s), 4 x 1024 x 1024 3.9.
 template <typename T, int MODE, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
     constexpr int N = VEC<T>, KC = 8 * N, U = 4, ROWS = 16 * MT, COLS = 16 * NT;
@@ -930,6 +942,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
 // outputs that are not stored); beyond the reduction's end both operands read
 // zeros, and the K-tiles are rounded up to an even number of at least 4; only
 // the first two and the last two can be partial.
+//
+// Bound by the matrix instructions while the reduction runs (1.3 us a K-tile of
+// all CUs, 1.65 PFLOP/s of 2.5) and by the epilogue's stores at its end: some 12
+// us of a tile are beside the K-tiles, of which half is the burst of stores.  bf16
+// 8192 x 8192 x 8192 738 us (1.49 PFLOP/s), 32000 x 1024 x 12544 with ReLU 580 to
+// 620 (1.33 to 1.42), 16128 x 4096 x 1024 137 to 145 (0.93 to 0.99).
 constexpr int BIG = 256, BIG_BUF = 65536, BIG_LDS = 2 * BIG_BUF, BIG_HALF = 16384;
 
 // a lane's part in staging and reading one operand
@@ -971,7 +989,9 @@ template <typename T, bool TR, bool ISB> struct BigOperand {
 
 // Tile id of a product.  (Persistent workgroups, which had the next tile's
 // first K-tiles on their way during the epilogue, spilled around it and were
-// 5 to 45 % slower than a workgroup per tile.)
+// 5 to 45 % slower than a workgroup per tile; tiles of 256 x 128 with K-tiles of
+// 32, two on a CU, took 177 us for 16128 x 4096 x 1024 where these took 164, and
+// 1028 for 32000 x 1024 x 12544 where these took 584.)
 template <typename T, bool TA, bool TB, int MODE>
 __device__ __forceinline__ void big_product(const Args &g, char *lds, int id) {
     Where w;
@@ -1176,7 +1196,8 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_forward(Args g) {
     run_tile<T, false, false, MODE, KIND>(g, lds, blockIdx.x);
 }
 // dW's tiles and dx's in one launch: they need nothing of each other, and
-// either alone often leaves part of the CUs without a tile.  Of dW's nw tiles
+// either alone often leaves part of the CUs without a tile (8192 x 4096 x 1024
+// bf16: 111 us for both, 2 x 69 GFLOP at 1.24 PFLOP/s).  Of dW's nw tiles
 // the `first` ones come before dx's, whose reduction is x.R: those that reduce
 // more (grouped: of the groups with more rows).  The bias's blocks come last.
 template <typename T, bool GROUPED, int KIND>
@@ -1200,7 +1221,8 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int 
 }
 
 // The slices' partial sums, added in their order (no atomics: the same result
-// on every call), and the epilogue; one thread per 16 bytes of output.
+// on every call), and the epilogue; one thread per 16 bytes of output.  Bound by
+// HBM: four slices of 4096 x 1024 8.8 us (8.6 TB/s from the L2s and beyond).
 template <typename T>
 __global__ __launch_bounds__(256) void k_product_join(Args g) {
     constexpr int N = VEC<T>;
@@ -1222,8 +1244,11 @@ __global__ __launch_bounds__(256) void k_product_join(Args g) {
 
 // dz = dy act'(z) in T, and the column sums of dz before that rounding.  A
 // workgroup takes one chunk of `rows` rows of a group by 32 pieces of 16 bytes;
-// its sums go to part[chunk][N], and k_bias_join adds a group's chunks.  Bound
-// by HBM.
+// its sums go to part[chunk][N], and bias_join adds a group's chunks.  Bound by
+// HBM: 8192 x 4096 bf16 GELU 44 us for its 201 MB (4.6 TB/s), 8000 x 2048 ReLU 17.4
+// (5.6 TB/s).  On its own, since both products take dz, each in another order:
+// in their loads it would be computed 4 to 16 times over and bar the direct way
+// to LDS.
 template <typename T>
 __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
     constexpr int W = VEC<T>, AT = 2;  // rows of a thread at once
