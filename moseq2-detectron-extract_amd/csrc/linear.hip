@@ -137,7 +137,8 @@ __device__ __forceinline__ float act_slope(float z, int act) {
         }
         case MDX_ACT_GELU_TANH: {
             const float s = tanh_gate(z);
-            return s + z * s * (1.f - s) * TANH_C * (1.f + 3.f * TANH_A * z * z);
+            // z^2 is cut where the gate has long been 0 or 1, so that it cannot overflow beside them
+            return s + z * s * (1.f - s) * TANH_C * (1.f + 3.f * TANH_A * fminf(z * z, 1e30f));
         }
         case MDX_ACT_SILU: {
             const float s = logistic(-LOG2E * z);

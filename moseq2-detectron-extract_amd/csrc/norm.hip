@@ -223,7 +223,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm(Args a) {
 // end.  Bound by HBM up to some 4000 columns (bf16 32000 x 1024 with the join 36 us,
 // 5.4 TB/s; 458752 x 256 139, 5.1), beyond by one workgroup's latency from row
 // to row: gamma, the sums and one row fill the registers, and nothing else runs
-// on the CU meanwhile (3000 x 12544 104 us, 2.2 TB/s).
+// on the CU meanwhile (2000 x 16384 70 us, 2.8 TB/s).
 template <typename T, int TPR, int NP>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_norm_backward(Args a) {
     using L = Rows<T, TPR, NP>;
@@ -467,9 +467,13 @@ static int backward_groups(long long rows, int D, int dtype) {
     if (!lay) return (int)std::min<long long>(64, std::max<long long>(1, rows / 16));
     const int slots = lay == 1 ? 16 : lay == 2 ? 8 : lay <= (dtype == 0 ? 6 : 5) ? 4 : 1;  // rows at once
     const int most = lay <= 3 || (dtype != 0 && lay == 6) ? 1024 : lay <= 7 ? 512 : 256;
-    // the shares (8 bytes a column, written and read) an eighth of the rows at most
-    const long long share = rows * (dtype == 0 ? 12 : 6) / 8 / 16;
-    return (int)std::max<long long>(1, std::min({ceil_div(rows, slots), (int64_t)most, (int64_t)std::max(share, 16ll)}));
+    // Each share is 8 bytes a column, written and read, so a workgroup should have
+    // several rows; but few workgroups wait for one row after the other.  128 of
+    // them, 256 where each still has 8 rows, more where each has 16 (bf16 200 x
+    // 16384: 16 workgroups 55 us, 128 36, 200 39; 600 x 16384: 32 75, 128 45, 256 49,
+    // 512 76; 2000 x 4096: 128 30, 256 24, 512 29; 8000 x 1500: 128 31, 256 22, 512 23).
+    const long long want = std::max({128ll, std::min(256ll, rows / 8), rows / 16});
+    return (int)std::max<long long>(1, std::min({(long long)ceil_div(rows, slots), (long long)most, want}));
 }
 
 template <typename T, int TPR, int NP> static void launch_forward(const Args &a, hipStream_t s) {

@@ -760,3 +760,26 @@ def test_grouped_few_rows(L, dt, E, per, N, K):
     for e, (s, t) in enumerate(sp):
         check_forward(y[s:t], pre[s:t], x[s:t], w[e], b[e], r[s:t], act, dt)
     assert (y[end:] == 0).all() and (pre[end:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_far_values(L, dt, act):
+    """Arguments near the ends of the type's range: every gate is 0 or 1 there,
+    and nothing overflows on the way.  (Rounding: none, 0 and 1 are exact.)"""
+    far = [1e4, 6e4] if dt == F16 else [1e4, 1e10, 1e19, 1e20, 3e38]
+    z = torch.tensor([-v for v in far] + far, dtype=dt, device="cuda").repeat(3, 5)
+    M, N = z.shape
+    x, w = torch.zeros(M, 8, dtype=dt, device="cuda"), torch.zeros(N, 8, dtype=dt, device="cuda")
+    want = z if act in (None, "none") else z.clamp(min=0)
+    assert torch.equal(L.linear(x, w, None, z, act), want)
+    got = L.linear_backward(torch.ones_like(z), x, w, z, act, need_residual=True).residual
+    assert torch.equal(got, torch.ones_like(z) if act in (None, "none") else (z > 0).to(dt))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("shape", [(129, 2048, 0, 0), (1030, 2049, 3, 1), (5, 8193, 0, 0), (300, 12544, 8, 0), (600, 16384, 0, 0),
+                                   (2100, 1500, 0, 0), (4100, 130, 1, 1)])
+def test_layer_norm_backward_shares(L, dt, shape):
+    """Rows on both sides of where more workgroups share the sums."""
+    test_layer_norm_backward(L, dt, shape)
