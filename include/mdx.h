@@ -574,6 +574,9 @@ enum {
     MDX_ACT_GELU_TANH = 3,  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
     MDX_ACT_SILU = 4        /* z / (1 + exp(-z)) */
 };
+/* Before its rounding an activation is within 16 * 2^-24 (float32) or 4e-5
+ * (16-bit types) of its value, far tails included; its slope within as much of
+ * the gate and of z times the gate's slope. */
 
 /* z = x w^T + bias + residual; out = act(z); pre (or NULL) = z.
  * x (M,K), w (N,K), bias [N] or NULL, residual (M,N) or NULL, out / pre (M,N).

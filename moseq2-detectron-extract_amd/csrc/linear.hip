@@ -94,87 +94,124 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T *p, int
 // ---- activations, in float32 ------------------------------------------------
 // On the hardware's exp2 and reciprocal (1 ulp each): with the library's erff,
 // tanhf and division the epilogue of a 256 x 256 tile took longer than its
-// product of 1024 terms.
-constexpr float LOG2E = 1.44269504088896341f;
-// 1 / (1 + exp2(u))
-__device__ __forceinline__ float logistic(float u) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u)); }
-// the normal distribution at z: *p its probability (1 + erf(z / sqrt 2)) / 2 by
-// formula 7.1.26 of Abramowitz and Stegun (erf to 1.5e-7), returned
-// exp(-z^2 / 2), which that formula needs and the density is made of
-__device__ __forceinline__ float normal_cdf(float z, float *p) {
-    const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.70710678118654752f) * fabsf(z));
-    const float e = __builtin_amdgcn_exp2f(z * z * (-0.5f * LOG2E));
-    const float c = e * t * (0.5f * 0.254829592f + t * (0.5f * -0.284496736f + t * (0.5f * 1.421413741f +
-                    t * (0.5f * -1.453152027f + t * (0.5f * 1.061405429f)))));
-    *p = z < 0.f ? c : 1.f - c;
-    return e;
+// product of 1024 terms.  That tile is for 16-bit outputs, to which GATE16 gives
+// some 15 bits; float32 outputs take GATE32, good to 16 * 2^-24 of the value, whose
+// exponents are formed in float64 (an exponent of 100 rounded to float32 alone is
+// off by 4e-6 of the power) and given to exp2 in two parts.
+enum Gates { GATE16, GATE32 };
+template <typename T> constexpr Gates GATES = sizeof(T) == 4 ? GATE32 : GATE16;
+constexpr double LOG2E = 1.4426950408889634;
+// the normal distribution at z <= 0 is exp(-z^2 / 2) times a smooth function of
+// |z|, taken as t = 1 / (1 + a |z|) times a polynomial that was fitted (minimax,
+// up to |z| = 14.5, where the product leaves the range of float32) to the
+// relative error, so that far tails keep their digits
+//   GATE16: a = 0.3, degree 5: 2.2e-5 of the tail, 2.2e-7 in all (3.5e-7 as computed)
+//   GATE32: a = 0.4 and t - 0.43, degree 8, from |z| = 1 on: 1e-8; below 1 the odd
+//           series' part z R(z^2) beside 1 / 2, whose degree 5 gives 1e-8
+constexpr float TAIL16[] = {0.12006758f, 0.113622055f, 0.145469342f, -0.0207057571f, 0.220405522f, -0.0788589624f};
+constexpr float TAIL32[] = {0.2594182808f,  0.31709961f,    0.2142576792f,   0.0003599896101f, -0.1069903019f,
+                            -0.01009159273f, 0.07743831973f, -0.00430055336f, -0.05770715095f};
+constexpr float CENTRE32[] = {0.3989422798f,   -0.06649034774f, 0.009973218223f,
+                              -0.001186034065f, 0.0001131538992f, -7.524209733e-06f};
+template <int N> __device__ __forceinline__ float polynomial(const float (&c)[N], float x) {
+    float v = c[N - 1];
+#pragma unroll
+    for (int k = N - 2; k >= 0; --k) v = fmaf(v, x, c[k]);
+    return v;
 }
-// the tanh form: (1 + tanh v) / 2 = 1 / (1 + exp(-2 v)), 2 v = C (z + A z^3)
-constexpr float TANH_C = 1.59576912160573071f, TANH_A = 0.044715f;
-__device__ __forceinline__ float tanh_gate(float z) {
-    return logistic(z * (-TANH_C * LOG2E + (-TANH_C * TANH_A * LOG2E) * (z * z)));
+// 2^u, u <= 0
+__device__ __forceinline__ float exp2_of(double u) {
+    u = fmax(u, -200.0);
+    const float hi = (float)u, e = __builtin_amdgcn_exp2f(hi);
+    return fmaf(e * (float)(u - (double)hi), 0.69314718056f, e);
+}
+// 1 / d, 1 <= d < 4
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.f), r, r);
+}
+// the normal distribution at z: *p its probability (1 + erf(z / sqrt 2)) / 2,
+// returned exp(-z^2 / 2), which that needs and the density is made of
+template <Gates G> __device__ __forceinline__ float normal_cdf(float z, float *p) {
+    const float m = fabsf(z);
+    if constexpr (G == GATE16) {
+        const float t = __builtin_amdgcn_rcpf(1.f + 0.3f * m);
+        const float e = __builtin_amdgcn_exp2f(z * z * (float)(-0.5 * LOG2E));
+        const float c = e * t * polynomial(TAIL16, t);
+        *p = z < 0.f ? c : 1.f - c;
+        return e;
+    } else {
+        const float e = exp2_of((double)z * z * (-0.5 * LOG2E));
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.4f, fminf(m, 1e4f), 1.f));
+        const float c = e * t * polynomial(TAIL32, t - 0.43f);
+        *p = m < 1.f ? fmaf(z, polynomial(CENTRE32, z * z), 0.5f) : z < 0.f ? c : 1.f - c;
+        return e;
+    }
+}
+// 1 / (1 + exp(-v)) and what it lacks to 1, v = z (silu) or 2 sqrt(2 / pi) (z + A z^3)
+// (the tanh form: (1 + tanh(v / 2)) / 2).  GATE16 gives 0 where exp(-v) passes the range.
+constexpr double TANH_C = 1.5957691216057308, TANH_A = 0.044715;
+template <Gates G, int ACT> __device__ __forceinline__ float logistic(float z, float *rest) {
+    if constexpr (G == GATE16) {
+        constexpr float c = (float)(-TANH_C * LOG2E), a = (float)(-TANH_C * TANH_A * LOG2E);
+        const float u = ACT == MDX_ACT_SILU ? (float)-LOG2E * z : z * (c + a * (z * z));
+        const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u));
+        *rest = 1.f - s;
+        return s;
+    } else {
+        const double x = z, v = ACT == MDX_ACT_SILU ? x : x * (TANH_C + TANH_C * TANH_A * (x * x));
+        const float e = exp2_of(-LOG2E * fabs(v)), r = reciprocal(1.f + e);
+        *rest = z < 0.f ? r : e * r;
+        return z < 0.f ? e * r : r;
+    }
 }
 
-__device__ __forceinline__ float act_value(float z, int act) {
-    switch (act) {
-        case MDX_ACT_RELU: return z < 0.f ? 0.f : z;  // NaN stays NaN
-        case MDX_ACT_GELU: {
-            float p;
-            normal_cdf(z, &p);
-            return z * p;
-        }
-        case MDX_ACT_GELU_TANH: return z * tanh_gate(z);
-        case MDX_ACT_SILU: return z * logistic(-LOG2E * z);
-        default: return z;
+template <Gates G, int ACT> __device__ __forceinline__ float act_value(float z) {
+    float p;
+    if constexpr (ACT == MDX_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays NaN
+    if constexpr (ACT == MDX_ACT_GELU) {
+        normal_cdf<G>(z, &p);
+        return z * p;
     }
-}
-__device__ __forceinline__ float act_slope(float z, int act) {
-    switch (act) {
-        case MDX_ACT_GELU: {
-            float p;
-            const float e = normal_cdf(z, &p);
-            return p + z * e * 0.39894228040143268f;
-        }
-        case MDX_ACT_GELU_TANH: {
-            const float s = tanh_gate(z);
-            // z^2 is cut where the gate has long been 0 or 1, so that it cannot overflow beside them
-            return s + z * s * (1.f - s) * TANH_C * (1.f + 3.f * TANH_A * fminf(z * z, 1e30f));
-        }
-        case MDX_ACT_SILU: {
-            const float s = logistic(-LOG2E * z);
-            return s * (1.f + z * (1.f - s));
-        }
-        default: return 1.f;
-    }
-}
-// a whole piece: the activation is chosen once, not for each element
-template <int ACT, int N> __device__ __forceinline__ void apply(float (&v)[N]) {
-#pragma unroll
-    for (int q = 0; q < N; ++q) v[q] = act_value(v[q], ACT);
-}
-template <int N> __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
-    switch (act) {
-        case MDX_ACT_RELU: return apply<MDX_ACT_RELU>(v);
-        case MDX_ACT_GELU: return apply<MDX_ACT_GELU>(v);
-        case MDX_ACT_GELU_TANH: return apply<MDX_ACT_GELU_TANH>(v);
-        case MDX_ACT_SILU: return apply<MDX_ACT_SILU>(v);
-    }
+    return z * logistic<G, ACT>(z, &p);
 }
 // dy act'(z); ReLU selects, so that an infinite gradient of a closed unit is dropped
-__device__ __forceinline__ float act_grad(float dy, float z, int act) {
-    if (act == MDX_ACT_RELU) return z > 0.f ? dy : 0.f;
-    return dy * act_slope(z, act);
+template <Gates G, int ACT> __device__ __forceinline__ float act_grad(float dy, float z) {
+    float p;
+    if constexpr (ACT == MDX_ACT_RELU) return z > 0.f ? dy : 0.f;
+    if constexpr (ACT == MDX_ACT_GELU) {
+        const float e = normal_cdf<G>(z, &p);
+        return dy * (p + z * e * 0.39894228040143268f);
+    }
+    const float s = logistic<G, ACT>(z, &p);
+    if constexpr (ACT == MDX_ACT_SILU) return dy * (s * (1.f + z * p));
+    // z^2 is cut where the gate has long been 0 or 1, so that it cannot overflow beside them
+    return dy * (s + z * s * p * (float)TANH_C * (1.f + (float)(3 * TANH_A) * fminf(z * z, 1e30f)));
 }
-template <int ACT, int N> __device__ __forceinline__ void apply_grad(float (&v)[N], const float (&z)[N]) {
+// a whole piece: the activation is chosen once, not for each element
+template <Gates G, int ACT, int N> __device__ __forceinline__ void apply(float (&v)[N]) {
 #pragma unroll
-    for (int q = 0; q < N; ++q) v[q] = act_grad(v[q], z[q], ACT);
+    for (int q = 0; q < N; ++q) v[q] = act_value<G, ACT>(v[q]);
 }
-template <int N> __device__ __forceinline__ void apply_act_grad(float (&v)[N], const float (&z)[N], int act) {
+template <Gates G, int N> __device__ __forceinline__ void apply_act(float (&v)[N], int act) {
     switch (act) {
-        case MDX_ACT_RELU: return apply_grad<MDX_ACT_RELU>(v, z);
-        case MDX_ACT_GELU: return apply_grad<MDX_ACT_GELU>(v, z);
-        case MDX_ACT_GELU_TANH: return apply_grad<MDX_ACT_GELU_TANH>(v, z);
-        case MDX_ACT_SILU: return apply_grad<MDX_ACT_SILU>(v, z);
+        case MDX_ACT_RELU: return apply<G, MDX_ACT_RELU>(v);
+        case MDX_ACT_GELU: return apply<G, MDX_ACT_GELU>(v);
+        case MDX_ACT_GELU_TANH: return apply<G, MDX_ACT_GELU_TANH>(v);
+        case MDX_ACT_SILU: return apply<G, MDX_ACT_SILU>(v);
+    }
+}
+template <Gates G, int ACT, int N> __device__ __forceinline__ void apply_grad(float (&v)[N], const float (&z)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) v[q] = act_grad<G, ACT>(v[q], z[q]);
+}
+template <Gates G, int N>
+__device__ __forceinline__ void apply_act_grad(float (&v)[N], const float (&z)[N], int act) {
+    switch (act) {
+        case MDX_ACT_RELU: return apply_grad<G, MDX_ACT_RELU>(v, z);
+        case MDX_ACT_GELU: return apply_grad<G, MDX_ACT_GELU>(v, z);
+        case MDX_ACT_GELU_TANH: return apply_grad<G, MDX_ACT_GELU_TANH>(v, z);
+        case MDX_ACT_SILU: return apply_grad<G, MDX_ACT_SILU>(v, z);
     }
 }
 
@@ -403,7 +440,7 @@ __device__ __forceinline__ void finish(const Args &g, long long ooff, Row i, int
 #pragma unroll
         for (int q = 0; q < N; ++q) v[q] += (float)r.e[q];
     if (g.pre) store_row<T, N>(reinterpret_cast<T *>(g.pre) + i.at(g.ldp) + j, n, v);
-    apply_act(v, g.act);
+    apply_act<GATES<T>>(v, g.act);
     store_row<T, N>(reinterpret_cast<T *>(g.out) + ooff + i.at(g.ldo) + j, n, v);
 }
 template <typename T> __device__ __forceinline__ u4 load_residual(const Args &g, Row i, int j) {
@@ -1277,7 +1314,7 @@ __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
             }
 #pragma unroll
             for (int k = 0; k < AT; ++k) {
-                if (!tail) apply_act_grad(v[k], w[k], g.act);
+                if (!tail) apply_act_grad<GATES<T>>(v[k], w[k], g.act);
                 if (g.dz && r + 8 * k < r1) store_row<T, W>(dz + (r + 8 * k) * g.lddz, n, v[k]);
 #pragma unroll
                 for (int q = 0; q < W; ++q) sum[q] += v[k][q];

@@ -783,3 +783,38 @@ def test_far_values(L, dt, act):
 def test_layer_norm_backward_shares(L, dt, shape):
     """Rows on both sides of where more workgroups share the sums."""
     test_layer_norm_backward(L, dt, shape)
+
+
+def gate(z, act):
+    """What z is multiplied with by an activation of z <= 0 or more, to the last digits of the far tails."""
+    if act == "gelu":
+        return 0.5 * torch.special.erfc(z * -0.5 ** 0.5)
+    if act == "gelu_tanh":
+        z = math.sqrt(8 / math.pi) * (z + 0.044715 * z ** 3)
+    return torch.special.expit(z)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("act,low", [("gelu", -12.0), ("gelu_tanh", -9.0), ("silu", -80.0)])
+def test_activation_tails(L, dt, act, low):
+    """Relative errors: an activation's far negative tail keeps its digits.
+
+    float32: the fits are good to 1e-8, their float32 evaluation to 6 v (emulated), exp2 and the reciprocal
+    to one step (2 v) each, of which the latter enters twice, and the product with z adds v: below 16 v.
+    16 bits: 2.8e-5 (the fit's 2.2e-5 with its roundings; exponents up to 126 rounded three times to float32
+    give 1.6e-5), a few steps of float32 beside it: below 4e-5, and the output's rounding.  The slope is the
+    gate and z times the density, each to that."""
+    z = torch.cat([torch.linspace(low, 0, 4001), torch.linspace(0, 12, 1001)[1:]]).to(dt)
+    Z = z.double()
+    t, u = (16 * V, 0.0) if dt == F32 else (4e-5, unit(dt))
+    x, w = z[:, None].contiguous().cuda(), torch.ones(1, 1, dtype=dt, device="cuda")
+    y = L.linear(x, w, None, None, act)
+    want = Z * gate(Z, act)
+    within(y[:, 0], want, (t + u) * want.abs() + sub(dt), act)
+    s, c = gate(Z, act), gate(-Z, act)
+    if act == "gelu":
+        part = Z * torch.exp(-Z * Z / 2) / math.sqrt(2 * math.pi)
+    else:
+        part = Z * s * c * (1 if act == "silu" else math.sqrt(8 / math.pi) * (1 + 3 * 0.044715 * Z * Z))
+    got = L.linear_backward(torch.ones_like(x), x, w, x, act, need_x=False, need_weight=False, need_residual=True)
+    within(got.residual[:, 0], s + part, t * (s + part.abs()) + u * (s + part).abs() + sub(dt), act)
