@@ -589,8 +589,11 @@ int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const flo
                int64_t ldr, int64_t M, int N, int K, int act, int dtype, void *pre, int64_t ldp, void *out, int64_t ldo,
                void *workspace, int64_t workspace_bytes, mdx_stream_t stream);
 /* Its gradients, each computed where its pointer is not NULL: dz = grad act'(pre),
- * rounded to dtype; dx = dz w, dw = dz^T x, dres = dz, dbias = the column sums
- * of dz before that rounding.  pre may be NULL for MDX_ACT_NONE.  dres may be
+ * rounded to dtype before dx = dz w and dw = dz^T x are taken; dres = dz, dbias =
+ * the column sums of dz before that rounding.  In 16-bit types that rounding makes
+ * dx and dw 1.4 times as inexact as their own alone; in float16 a dz beyond 65504
+ * is infinite and one below 3e-8 zero, as between separate float16 layers.  float32
+ * operands keep all of dz.  pre may be NULL for MDX_ACT_NONE.  dres may be
  * grad's own buffer (same lddr).  workspace: at least
  * mdx_linear_backward_workspace_bytes (which gradients are needed as flags).
  * Sums are taken in a fixed order: a call repeats bit for bit. */

@@ -12,8 +12,12 @@
 // so no operand is ever transposed in memory.  Sums are float32 in the matrix
 // instructions; each output is rounded once.  dz is rounded to the operands'
 // type before the two products, since the matrix instructions take nothing
-// wider: a term is off by half a step of that type at most (bf16 gradients are
-// off by 0.0023 of their size on the whole, where rounded outputs alone give 0.0017).
+// wider: a term is off by half a step of that type at most (bf16 gradients of
+// 8192 x 4096 x 1024 GELU are off by 0.0023 of their size on the whole, where rounded
+// outputs alone give 0.0017; fp16 999 x 517 x 1001 SiLU 2.9e-4 and 2.1e-4).  A dz in
+// two parts would keep the rest for twice the products' time (8192 x 4096 x 1024:
+// 111 us); between separate layers of the type it is rounded just so.  In fp16
+// it shares the type's range: beyond 65504 infinite, below 2^-25 zero.
 #include "common.h"
 
 #include <algorithm>

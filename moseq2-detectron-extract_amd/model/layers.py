@@ -298,7 +298,9 @@ def linear_backward(grad, x, weight, pre=None, activation=None, *, need_x: bool 
     x = dz @ weight, weight = dz.T @ x, bias = dz's sum over the rows
     (float32), residual = dz (grad itself when there is no activation).  pre:
     what linear(..., return_pre=True) returned; not needed without an
-    activation.  dz is rounded to x's dtype where it enters the products."""
+    activation.  dz is rounded to x's dtype where it enters the products (in
+    float16 infinite beyond 65504 and zero below 3e-8, as between separate
+    float16 layers: scale the loss); float32 operands keep all of it."""
     return _backward(grad, x, None, weight, pre, activation, need_x, need_weight, need_bias, need_residual)
 
 

@@ -818,3 +818,22 @@ def test_activation_tails(L, dt, act, low):
         part = Z * s * c * (1 if act == "silu" else math.sqrt(8 / math.pi) * (1 + 3 * 0.044715 * Z * Z))
     got = L.linear_backward(torch.ones_like(x), x, w, x, act, need_x=False, need_weight=False, need_residual=True)
     within(got.residual[:, 0], s + part, t * (s + part.abs()) + u * (s + part).abs() + sub(dt), act)
+
+
+def test_float16_range_of_dz(L):
+    """dz enters the float16 products rounded to float16: past 65504 it is infinite, below 2^-25 zero, and the
+    bias's gradient is summed before that.  float32 operands keep both.  Bounds: 4e-5 and 16 v of the slope's
+    two parts (test_activation_tails), and v for each product and sum."""
+    z = torch.tensor([[1.5, -0.5]], dtype=F16, device="cuda")
+    dy = torch.tensor([[65504.0, 2.0 ** -24]], dtype=F16, device="cuda")  # slopes 1.127 and 0.132
+    x = torch.full((1, 8), 2.0 ** -10, dtype=F16, device="cuda")
+    w = torch.tensor([[2.0 ** -10] * 8, [1.0] * 8], dtype=F16, device="cuda")
+    got = L.linear_backward(dy, x, w, z, "gelu", need_bias=True, need_residual=True)
+    assert got.residual.tolist() == [[float("inf"), 0.0]] and got.x.isinf().all()
+    assert got.weight[0].isinf().all() and (got.weight[1] == 0).all()
+    Z, DY, W = z.double().cpu(), dy.double().cpu(), w.double().cpu()
+    want, size = DY * slope(Z, "gelu"), DY * (gate(Z, "gelu") + (Z * torch.exp(-Z * Z / 2)).abs() / math.sqrt(2 * math.pi))
+    within(got.bias, want[0], (4e-5 + 2 * V) * size[0], "db")
+    full = L.linear_backward(dy.float(), x.float(), w.float(), z.float(), "gelu", need_residual=True)
+    within(full.residual, want, 18 * V * size, "dr")
+    within(full.x, want @ W, 24 * V * (size @ W), "dx")
