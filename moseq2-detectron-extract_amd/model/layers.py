@@ -19,13 +19,15 @@ synchronisation, so the calls can be captured into a graph.  ``bias``,
 ``gamma`` / ``beta`` and their gradients are float32, everything else has the
 input's dtype.  Leading axes are flattened; rows may be strided, other layouts
 are copied first.  Gradients are explicit calls: tensors that require grad are
-refused outside ``torch.no_grad()``, since no graph is recorded.
+refused outside ``torch.no_grad()``, since no graph is recorded; so are tensors
+with a forward-mode tangent, and calls under a tracer.
 """
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import call
 
@@ -61,6 +63,8 @@ class LayerNormGrads(NamedTuple):
 _Tensor, _strided = torch.Tensor, torch.strided
 _stream = torch._C._cuda_getCurrentRawStream
 _current = torch._C._cuda_getDevice
+_tracing = torch._C._get_tracing_state
+_mode, _PROXY = torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
 
 
 def _activation(name) -> int:
@@ -100,11 +104,19 @@ def _check_input(what: str, x: torch.Tensor, dims: int = 1) -> None:
 
 
 def _check_run(x: torch.Tensor, *others) -> None:
+    """Refuses what would be lost without a word: derivatives in either mode,
+    and a call that a tracer records as the allocation of its outputs."""
     if torch.is_grad_enabled():
         for t in (x, *others):
             if t is not None and t.requires_grad:
                 raise ValueError("a tensor requires grad: call under torch.no_grad() and take the gradients with the "
                                  "_backward function (no autograd graph is recorded)")
+    if forward_ad._current_level >= 0:
+        for t in (x, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("a tensor carries a tangent: there is no forward-mode derivative")
+    if _tracing() is not None or _mode(_PROXY) is not None:
+        raise RuntimeError("the call cannot be traced: capture it into a CUDA graph instead")
     if not x.is_cuda:
         raise ValueError("tensors must be on the GPU; there is no CPU fallback")
 
@@ -180,6 +192,11 @@ def _laid(t: Optional[torch.Tensor]):
         return t, width
     r = _rows(t)
     return r, max(r.stride(0), width)
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t, or a contiguous copy of what it stands for."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -263,8 +280,8 @@ def _forward(x, counts, weight, bias, residual, activation, return_pre, out):
         with torch.cuda.device(x.device):
             return _forward(x, counts, weight, bias, residual, activation, return_pre, out)
     xr, ldx = _laid(x)
-    w, ldw = (weight.contiguous(), K) if grouped else _laid(weight)
-    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    w, ldw = (_dense(weight), K) if grouped else _laid(weight)
+    b = _dense(bias)
     r, ldr = _laid(residual)
     fresh = out is None
     if fresh:
@@ -349,7 +366,7 @@ def _backward(grad, x, counts, weight, pre, activation, need_x, need_weight, nee
     if need_x or need_weight or need_bias or own:
         xr, ldx = _laid(x)
         gr, ldg = _laid(grad)
-        w, ldw = (weight.contiguous(), K) if grouped else _laid(weight)
+        w, ldw = (_dense(weight), K) if grouped else _laid(weight)
         z, ldz = _laid(pre) if act else (None, 0)
         dt, stream = _DTYPES[x.dtype], _stream(x.get_device())
         flags = (bool(need_x), bool(need_weight), bool(need_bias), bool(own))
@@ -388,8 +405,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, return_stats: bo
         with torch.cuda.device(x.device):
             return layer_norm(x, weight, bias, eps, return_stats=return_stats, out=out)
     xr, ldx = _laid(x)
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    w = _dense(weight)
+    b = _dense(bias)
     if out is None:
         o = out = x.new_empty(x.shape)
         ldo = D
@@ -430,9 +447,8 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, need_x: bool = True
     if need_x or need_weight or need_bias:
         xr, ldx = _laid(x)
         gr, ldg = _laid(grad)
-        m = mean if mean.is_contiguous() else mean.contiguous()
-        r = rstd if rstd.is_contiguous() else rstd.contiguous()
-        w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+        m, r = _dense(mean), _dense(rstd)
+        w = _dense(weight)
         rows, dt = x.numel() // D, _DTYPES[x.dtype]
         nbytes = call("mdx_layer_norm_backward_workspace_bytes", rows, D, dt) if need_weight or need_bias else 0
         ws = _workspace(nbytes, x)

@@ -230,3 +230,45 @@ def test_c_entry_refuses_too_many_bias_columns(mdx):
     rc, text = _refused("mdx_grouped_linear_backward", p, 1 << 20, p, 1, p, nul, 0, p, 4096, 4, 1 << 20, 1, 0, 3, nul, 1,
                         nul, p, nul, 0, 1, p, 1 << 50, nul)
     assert rc == -1 and "columns of bias" in text, (rc, text)
+
+
+def every_call(L, x, dtype=F32):
+    """Calls of all entries that get x (4, 8) as their first or second tensor, by name."""
+    w, c, s = z(3, 8, dtype=dtype), z(2, dtype=I32), z(4, dtype=F32)
+    dy = z(4, 3, dtype=dtype)
+    return {"linear": lambda: L.linear(x, w), "grouped_linear": lambda: L.grouped_linear(x, c, z(2, 3, 8, dtype=dtype)),
+            "linear_backward": lambda: L.linear_backward(dy, x, w),
+            "grouped_linear_backward": lambda: L.grouped_linear_backward(dy, x, c, z(2, 3, 8, dtype=dtype)),
+            "layer_norm": lambda: L.layer_norm(x), "layer_norm_backward": lambda: L.layer_norm_backward(z(4, 8, dtype=dtype), x, s, s)}
+
+
+def test_tangents_are_refused(L):
+    """A forward-mode tangent would be lost; requires_grad does not show it."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(z(4, 8, dtype=F32), torch.ones(4, 8))
+        for name, f in every_call(L, x).items():
+            with pytest.raises(ValueError, match="tangent"):
+                f()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # which leaves tangents alone
+                f()
+        b = forward_ad.make_dual(z(3, dtype=F32), torch.ones(3))
+        with pytest.raises(ValueError, match="tangent"):
+            L.linear(z(4, 8, dtype=F32), z(3, 8, dtype=F32), b)
+        for f in every_call(L, z(4, 8, dtype=F32)).values():  # a level without tangents is no matter
+            with pytest.raises(ValueError, match="GPU"):
+                f()
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda a: L.layer_norm(a), (z(4, 8, dtype=F32),), (torch.ones(4, 8),))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracers_are_refused(L):
+    """A trace would hold the allocation of the outputs and not the call."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for name in every_call(L, z(4, 8, dtype=F32)):
+        f = lambda a: every_call(L, a)[name]()  # noqa: B023, E731
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (z(4, 8, dtype=F32),))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(z(4, 8, dtype=F32))
