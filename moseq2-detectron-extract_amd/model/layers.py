@@ -131,6 +131,10 @@ def _rows(t: torch.Tensor, copy: bool = True) -> Optional[torch.Tensor]:
     distance of at least the width; a copy where its layout allows no such
     view (None with copy=False)."""
     width = t.shape[-1]
+    if t.is_neg():  # of a conjugate's imaginary part: the memory holds -t
+        if not copy:
+            return None
+        t = t.resolve_neg()
     if t.is_contiguous():
         r = t if t.dim() == 2 else t.view(-1, width)
         if r.stride(0) == width:
@@ -188,7 +192,7 @@ def _laid(t: Optional[torch.Tensor]):
     if t is None:
         return None, 0
     width = t.shape[-1]
-    if t.is_contiguous():
+    if t.is_contiguous() and not t.is_neg():
         return t, width
     r = _rows(t)
     return r, max(r.stride(0), width)
@@ -196,7 +200,9 @@ def _laid(t: Optional[torch.Tensor]):
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """t, or a contiguous copy of what it stands for."""
-    return t if t is None or t.is_contiguous() else t.contiguous()
+    if t is None or t.is_contiguous() and not t.is_neg():
+        return t
+    return t.resolve_neg().contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):

@@ -272,3 +272,17 @@ def test_tracers_are_refused(L):
             torch.jit.trace(f, (z(4, 8, dtype=F32),))
         with pytest.raises(RuntimeError, match="traced"):
             make_fx(f)(z(4, 8, dtype=F32))
+
+
+def test_negative_views(L):
+    """The imaginary part of a conjugate is a view that stands for -1 times its memory."""
+    for shape in ((1, 1), (5, 1), (3, 4)):
+        c = torch.arange(1, 1 + 2 * shape[0] * shape[1], dtype=F32).view(*shape, 2)
+        t = torch.view_as_complex(c).conj().imag
+        want = -c[..., 1]
+        assert t.is_neg()
+        for r in (L._rows(t), L._laid(t)[0], L._dense(t)):
+            assert not r.is_neg() and r.is_contiguous() and torch.equal(r.view(shape), want)
+        assert L._laid(t)[1] == shape[1] and L._rows(t, copy=False) is None
+    t = torch._neg_view(torch.ones(3, 4))  # contiguous
+    assert torch.equal(L._laid(t)[0], -torch.ones(3, 4)) and not L._laid(t)[0].is_neg() and not L._dense(t).is_neg()

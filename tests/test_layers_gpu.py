@@ -837,3 +837,21 @@ def test_float16_range_of_dz(L):
     full = L.linear_backward(dy.float(), x.float(), w.float(), z.float(), "gelu", need_residual=True)
     within(full.residual, want, 18 * V * size, "dr")
     within(full.x, want @ W, 24 * V * (size @ W), "dx")
+
+
+def test_negative_views(L):
+    """Operands that are lazily negated views (a conjugate's imaginary part)."""
+    c = torch.view_as_complex(normal(gen(31), 6, 1, 2)).cuda()
+    x, plain = c.conj().imag, -c.imag.contiguous()
+    assert x.is_neg()
+    w, b = torch.full((1, 1), 2.0, device="cuda"), torch.full((1,), 0.5, device="cuda")
+    assert torch.equal(L.linear(x, w, b, x), L.linear(plain, w, b, plain))
+    n, m = c[:1].conj().imag, -c[:1].imag.contiguous()  # (1, 1): also contiguous
+    assert n.is_neg() and n.is_contiguous()
+    assert torch.equal(L.linear(n, n, n[0], n), L.linear(m, m, m[0], m))
+    for got, want in zip(L.linear_backward(x, x, n, x, "silu", need_bias=True, need_residual=True),
+                         L.linear_backward(plain, plain, m, plain, "silu", need_bias=True, need_residual=True)):
+        assert torch.equal(got, want)
+    assert torch.equal(L.layer_norm(x, n[0], n[0]), L.layer_norm(plain, m[0], m[0]))
+    with pytest.raises(ValueError, match="rows"):
+        L.linear(plain, w, out=x)
