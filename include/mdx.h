@@ -562,7 +562,9 @@ int mdx_heatmaps_to_keypoints(const float *maps, const float *boxes, const int *
  * are row-major; ld* is the distance between rows in elements, at least the
  * row's length, with any alignment (rows of whole 16-byte pieces at 16-byte
  * addresses take the faster kernels); a workspace is 16-byte aligned.  At most
- * 2^31 - 65537 rows or columns.  An output must not overlap an input, except
+ * 2^31 - 65537 rows or columns; refused are outputs that 2^24 tiles of 128 x 128
+ * do not cover, and dbias of 2^27 columns or more over all groups (each group's
+ * rounded up to 16).  An output must not overlap an input, except
  * where it is exactly that buffer and the call says so.  No entry
  * allocates or synchronises: all can be captured into a graph, and calls on
  * several streams run side by side on workspaces of their own.

@@ -1340,6 +1340,8 @@ __global__ __launch_bounds__(256, 4) void k_act_backward(ActArgs g) {
 }
 // ---- host ---------------------------------------------------------------
 constexpr int CUS = 256;  // of an MI355X
+// a launch has fewer than 2^32 threads
+static bool fits(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
 
 struct Shape {
     long long T;  // rows
@@ -1352,8 +1354,8 @@ struct Shape {
 // reduction, and how many of it there are (grouped: on average).
 struct Load {
     long long I, J, R, groups;
-    bool red, split;  // grouped reduction; the reduction may be split
-};  // (of two, the first may be)
+    bool red, ragged, split;  // grouped reduction; grouped rows; the reduction may be split
+};                            // (of two, the first may be)
 struct Choice {
     int kind, splits;  // splits of each load that may be split
     double us;
@@ -1380,24 +1382,27 @@ static Cost cost_of(int kind, int es) {
 // the tiles, and of the join.  (1000 x 1024 x 12544: fp32 128-wide tiles in 8
 // slices 205 us, in 4 216, 64-wide in 2 222; bf16 64-wide in 2 slices 46, 128-wide
 // in 4 47, 256-wide in 8 51.)
+// A kernel whose launch would have too many threads is left out: narrow outputs
+// of more than 5e8 rows go to larger tiles than their work asks for.
 static Choice choose(const Load *loads, int n, int es, bool aligned, long long most_part) {
     Choice best{REG64, 1, 1e30};
     for (int kind = aligned ? (es == 2 ? LARGE : DMA128) : REG128; kind <= (aligned ? DMA64 : REG64); ++kind) {
         const Cost c = cost_of(kind, es);
         const int side = tile_side(kind);
         for (const int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
-            long long tiles[2], steps[2], all = 0, part = 0;
-            bool fits = true;
+            long long tiles[2], steps[2], all = 0, part = 0, most = 0;
+            bool enough = true;  // steps in a slice
             for (int k = 0; k < n; ++k) {
                 const Load &l = loads[k];
                 const int s = l.split ? splits : 1;
                 steps[k] = std::max<long long>(1, ceil_div(ceil_div(l.R * es, 128), s));
-                if (s > 1 && steps[k] < 4) fits = false;
+                if (s > 1 && steps[k] < 4) enough = false;
                 tiles[k] = ceil_div(l.I, side) * ceil_div(l.J, side) * l.groups * s;
                 all += tiles[k];
+                most += l.ragged ? (ceil_div(l.I * l.groups, side) + l.groups + 1) * ceil_div(l.J, side) : tiles[k];
                 if (s > 1) part += 4 * s * l.I * l.J * (l.red ? l.groups : 1);
             }
-            if (!fits || part > most_part) break;
+            if (!enough || part > most_part || !fits(most, tile_threads(kind))) break;
             const long long here = std::min<long long>(c.slots, std::max<long long>(1, ceil_div(all, CUS)));
             const double step = std::max(c.alone, here * c.shared);
             double work = 0, longest = 0;
@@ -1416,7 +1421,7 @@ static Choice choose(const Load *loads, int n, int es, bool aligned, long long m
 }
 static Load forward_load(const Shape &p) {
     const long long E = std::max(p.E, 1);
-    return Load{ceil_div(p.T, E), p.N, p.K, E, false, p.E == 0};
+    return Load{ceil_div(p.T, E), p.N, p.K, E, false, p.E > 0, p.E == 0};
 }
 // bytes of partial sums of a forward call; nothing in grouped ones is split
 static long long part_bytes(long long splits, long long E, long long I, long long J) {
@@ -1445,7 +1450,7 @@ static bool pieces(const void *p, long long ld, long long group, long long lengt
 static int set_tiles(Args &g, int mode, int bi, int bj, int threads, long long &n) {
     const long long ti = ceil_div(g.I, bi) + (mode == GROUP_ROWS ? g.E + 1 : 0), tj = ceil_div(g.J, bj);
     n = ti * tj * (mode == GROUP_RED ? g.E : 1) * g.splits;
-    MDX_REQUIRE(n * threads < (1ll << 31), "mdx_linear: too many output tiles");
+    MDX_REQUIRE(fits(n, threads), "mdx_linear: too many output tiles");
     g.ti = (int)ti;
     g.tj = (int)tj;
     return MDX_OK;
@@ -1480,7 +1485,7 @@ static int launch_backward(Args w, Args x, const ActArgs &sums, float *db, hipSt
         if (x.out)
             if (int rc = set_tiles(x, GROUPED ? GROUP_ROWS : DENSE, side, side, threads, nx)) return rc;
         const long long nb = db ? ceil_div(bias_units(sums), BIAS_UNITS) : 0;
-        MDX_REQUIRE((nw + nx + nb) * threads < (1ll << 31), "mdx_linear_backward: too many output tiles");
+        MDX_REQUIRE(fits(nw + nx + nb, threads), "mdx_linear_backward: too many output tiles");
         // without both, or with more groups than a wave has lanes: dW's first
         const int first = !w.out || !x.out ? (int)nw
                           : GROUPED        ? w.E <= 64 ? -1 : (int)nw
@@ -1508,7 +1513,6 @@ static Few few_plan(long long rows, int E, long long N, long long K, int es) {
     f.waves = each >= 64 && tiles * f.splits <= 2 * CUS ? 16 : each >= 32 ? 8 : 4;
     return f;
 }
-template <typename T, bool GROUP> static int launch_join(const Args &g, hipStream_t s);
 template <typename T, int MODE, int MT, int NT> static int launch_few(Args g, int waves, hipStream_t s) {
     long long n;
     if (int rc = set_tiles(g, MODE, 16 * MT, 16 * NT, 64 * waves, n)) return rc;
@@ -1551,22 +1555,40 @@ static bool few_rows(const Shape &p, bool aligned) {
     const long long steps = ceil_div((long long)p.K * p.es(), 128);
     return p.T <= 16ll * p.E && p.T * (aligned ? 16 : 64) <= steps * p.E;
 }
+// how a forward call is computed
+struct Plan {
+    bool few;
+    Few f;
+    Choice c;
+    int splits() const { return few ? f.splits : c.splits; }
+};
+static Plan plan_forward(const Shape &p, bool aligned, long long most_part) {
+    Plan q{few_rows(p, aligned), {}, {}};
+    if (q.few) {
+        q.f = few_plan(ceil_div(p.T, std::max(p.E, 1)), p.E, p.N, p.K, p.es());
+        if (part_bytes(q.f.splits, 0, p.T, p.N) > most_part) q.f.splits = 1;
+        // of some 5e8 columns or more the tiles need fewer threads
+        const long long ti = p.E ? ceil_div(p.T, 16) + p.E + 1 : ceil_div(p.T, 16 * q.f.mt);
+        q.few = fits(ti * ceil_div(p.N, 16 * q.f.nt) * q.f.splits, 64 * q.f.waves);
+    }
+    if (!q.few) {
+        const Load l = forward_load(p);
+        q.c = choose(&l, 1, p.es(), aligned, most_part);
+    }
+    return q;
+}
 template <typename T, int MODE> static int forward(const Shape &p, Args g, int64_t ws_bytes, hipStream_t s) {
-    g.splits = 1;
     const int es = sizeof(T);
     const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
-    if (few_rows(p, al)) {
-        const Few f = few_plan(ceil_div(p.T, std::max(p.E, 1)), p.E, p.N, p.K, es);
-        if (f.splits > 1 && g.part && ws_bytes >= part_bytes(f.splits, 0, p.T, p.N)) g.splits = f.splits;
+    const Plan q = plan_forward(p, al, g.part ? ws_bytes : 0);
+    g.splits = q.splits();
+    if (q.few) {
         if constexpr (MODE == DENSE)
-            if (f.mt == 2)
-                return f.nt == 1 ? launch_few<T, MODE, 2, 1>(g, f.waves, s) : launch_few<T, MODE, 2, 2>(g, f.waves, s);
-        return f.nt == 1 ? launch_few<T, MODE, 1, 1>(g, f.waves, s) : launch_few<T, MODE, 1, 2>(g, f.waves, s);
+            if (q.f.mt == 2)
+                return q.f.nt == 1 ? launch_few<T, MODE, 2, 1>(g, q.f.waves, s) : launch_few<T, MODE, 2, 2>(g, q.f.waves, s);
+        return q.f.nt == 1 ? launch_few<T, MODE, 1, 1>(g, q.f.waves, s) : launch_few<T, MODE, 1, 2>(g, q.f.waves, s);
     }
-    const Load l = forward_load(p);
-    const Choice c = choose(&l, 1, es, al, g.part ? ws_bytes : 0);
-    g.splits = c.splits;
-    switch (c.kind) {
+    switch (q.c.kind) {
         case LARGE: return launch_forward<T, MODE, LARGE>(g, s);
         case DMA128: return launch_forward<T, MODE, DMA128>(g, s);
         case DMA64: return launch_forward<T, MODE, DMA64>(g, s);
@@ -1577,11 +1599,8 @@ template <typename T, int MODE> static int forward(const Shape &p, Args g, int64
 // room for the split that either kind of kernel chooses, aligned operands or not
 static long long forward_bytes(const Shape &p) {
     if (p.E) return 0;
-    if (few_rows(p, true)) return part_bytes(few_plan(p.T, 0, p.N, p.K, p.es()).splits, 0, p.T, p.N);
-    const Load l = forward_load(p);
     long long n = 0;
-    for (int al = 0; al < 2; ++al)
-        n = std::max(n, part_bytes(choose(&l, 1, p.es(), al, PART_MAX).splits, 0, p.T, p.N));
+    for (int al = 0; al < 2; ++al) n = std::max(n, part_bytes(plan_forward(p, al, PART_MAX).splits(), 0, p.T, p.N));
     return n;
 }
 
@@ -1608,8 +1627,8 @@ static BackPlan plan_backward(const Shape &p, bool need_x, bool need_w, bool nee
     const long long E = std::max(p.E, 1);
     // chosen for both products whichever are needed, so that a gradient's bits
     // do not depend on which others are asked for
-    const Load l[2] = {Load{p.N, p.K, ceil_div(p.T, E), E, true, true},
-                       Load{ceil_div(p.T, E), p.K, p.N, E, false, false}};
+    const Load l[2] = {Load{p.N, p.K, ceil_div(p.T, E), E, true, false, true},
+                       Load{ceil_div(p.T, E), p.K, p.N, E, false, p.E > 0, false}};
     q.products = choose(l, 2, p.es(), aligned, PART_MAX);
     q.dz = p.act != MDX_ACT_NONE && (need_x || need_w) && !need_r;
     q.rows = act_rows(p.T, p.N, p.dtype);

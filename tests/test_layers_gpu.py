@@ -855,3 +855,23 @@ def test_negative_views(L):
     assert torch.equal(L.layer_norm(x, n[0], n[0]), L.layer_norm(plain, m[0], m[0]))
     with pytest.raises(ValueError, match="rows"):
         L.linear(plain, w, out=x)
+
+
+@pytest.mark.parametrize("M", [6 * 10 ** 8, 12 * 10 ** 8])
+def test_narrow_outputs_of_many_rows(L, M):
+    """The most rows that a launch of the 64-wide tiles has threads for, and more than those: the weight is the
+    unit matrix, so that every product is exact."""
+    dt = BF16
+    x = torch.empty(M, 8, dtype=dt, device="cuda").normal_()
+    w = torch.eye(8, dtype=dt, device="cuda")
+    assert torch.equal(L.linear(x, w), x)
+    assert torch.equal(L.linear_backward(x, x, w, need_weight=False).x, x)
+
+
+def test_wide_output_of_one_row(L):
+    """More columns than the kernel of few rows has threads for."""
+    N = 54 * 10 ** 7
+    w = torch.empty(N, 8, dtype=BF16, device="cuda").normal_()
+    x = torch.zeros(1, 8, dtype=BF16, device="cuda")
+    x[0, 3] = 1
+    assert torch.equal(L.linear(x, w)[0], w[:, 3])
