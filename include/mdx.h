@@ -583,9 +583,10 @@ enum {
 /* z = x w^T + bias + residual; out = act(z); pre (or NULL) = z.
  * x (M,K), w (N,K), bias [N] or NULL, residual (M,N) or NULL, out / pre (M,N).
  * out may be the residual's own buffer (same ldo).  workspace: where few
- * output tiles would leave CUs idle, the reduction is split and joined through
- * mdx_linear_workspace_bytes bytes (0 = not split); with less it is not
- * split. */
+ * output tiles would leave CUs idle, the reduction is split into slices and
+ * joined through 4 M N bytes a slice; mdx_linear_workspace_bytes are enough for
+ * operands of any alignment (0 = not split).  With less than the slices take the
+ * reduction is not split and the workspace not touched. */
 int64_t mdx_linear_workspace_bytes(int64_t M, int N, int K, int dtype);
 int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const float *bias, const void *residual,
                int64_t ldr, int64_t M, int N, int K, int act, int dtype, void *pre, int64_t ldp, void *out, int64_t ldo,

@@ -1580,7 +1580,10 @@ static Plan plan_forward(const Shape &p, bool aligned, long long most_part) {
 template <typename T, int MODE> static int forward(const Shape &p, Args g, int64_t ws_bytes, hipStream_t s) {
     const int es = sizeof(T);
     const bool al = pieces(g.a, g.lda, 0, g.R, es) && pieces(g.b, g.ldb, g.gstride, g.R, es);
-    const Plan q = plan_forward(p, al, g.part ? ws_bytes : 0);
+    Plan q = plan_forward(p, al, PART_MAX);
+    // without room for the slices of that plan the reduction is not split at all,
+    // so that the result does not follow the workspace's size any closer
+    if (q.splits() > 1 && (!g.part || ws_bytes < part_bytes(q.splits(), 0, p.T, p.N))) q = plan_forward(p, al, 0);
     g.splits = q.splits();
     if (q.few) {
         if constexpr (MODE == DENSE)

@@ -875,3 +875,36 @@ def test_wide_output_of_one_row(L):
     x = torch.zeros(1, 8, dtype=BF16, device="cuda")
     x[0, 3] = 1
     assert torch.equal(L.linear(x, w)[0], w[:, 3])
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(1000, 512, 4096), (300, 256, 2048), (9, 40, 8192)])
+def test_c_entry_splits_whole_or_not(L, mdx, dt, M, N, K):
+    """mdx_linear with less workspace than its slices take splits nothing, however little is missing, and leaves
+    the workspace as it was; the result does not follow the size."""
+    from moseq2_detectron_extract_amd._lib import call
+    g = gen(16)
+    x, w = normal(g, M, K, dtype=dt).cuda(), normal(g, N, K, dtype=dt, scale=K ** -0.5).cuda()
+    P = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    code = {F32: 0, BF16: 3}[dt]
+    most = call("mdx_linear_workspace_bytes", M, N, K, code)
+    assert most % (4 * M * N) == 0 and most >= 8 * M * N
+
+    def run(nbytes):
+        out, ws = torch.empty(M, N, dtype=dt, device="cuda"), torch.full((most,), 255, dtype=torch.uint8, device="cuda")
+        call("mdx_linear", P(x), K, P(w), K, None, None, 0, M, N, K, 0, code, None, 0, P(out), N, P(ws), nbytes, None)
+        torch.cuda.synchronize()
+        check_forward(out, None, x.cpu(), w.cpu(), None, None, "none", dt)
+        return out, bool((ws == 255).all())
+    whole, untouched = run(most)
+    assert not untouched and torch.equal(whole, L.linear(x, w))
+    once, untouched = run(0)
+    assert untouched
+    seen = {}
+    for nbytes in range(2 * M * N, most + 1, 2 * M * N):
+        for n in (nbytes - 1, nbytes):
+            out, untouched = run(n)
+            seen[n] = untouched
+            assert torch.equal(out, once if untouched else whole), n
+    need = min(n for n, u in seen.items() if not u)  # one size on which it turns, that of whole slices
+    assert need % (4 * M * N) == 0 and all(u == (n < need) for n, u in seen.items()), seen
