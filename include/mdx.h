@@ -607,6 +607,20 @@ int mdx_linear_backward(const void *grad, int64_t ldg, const void *x, int64_t ld
                         int64_t lddx, void *dw, int64_t lddw, float *dbias, void *dres, int64_t lddr, void *workspace,
                         int64_t workspace_bytes, mdx_stream_t stream);
 
+/* The kernel and the slices of the reduction that a call takes, as kernel + 16 *
+ * slices: of the forward pass, or of a backward pass's products (slices of dw).
+ * E = 0: mdx_linear, else the grouped one with T rows; aligned: whether all
+ * operands' rows are whole 16-byte pieces at 16-byte addresses. */
+enum {
+    MDX_LINEAR_256 = 0,      /* 256 x 256 tiles */
+    MDX_LINEAR_128 = 1,      /* 128 x 128, 64 x 64, aligned operands */
+    MDX_LINEAR_64 = 2,
+    MDX_LINEAR_128_ANY = 3,  /* 128 x 128, 64 x 64, operands of any alignment */
+    MDX_LINEAR_64_ANY = 4,
+    MDX_LINEAR_FEW = 5       /* few rows, any alignment */
+};
+int mdx_linear_plan(int E, int64_t T, int N, int K, int dtype, int aligned, int backward);
+
 /* The same layer with E weights over ragged groups of rows: rows of x (T,K)
  * lie group by group, counts [E] (int32, on the device, never read by the
  * host) of them each; w (E,N,K) and bias [E][N] are contiguous.  A negative

@@ -108,6 +108,7 @@ SIGNATURES = {
     "mdx_model_get_policy": (I32, [P, P]),
     "mdx_linear_workspace_bytes": (I64, [I64, I32, I32, I32]),
     "mdx_linear": (I32, [P, I64, P, I64, P, P, I64, I64, I32, I32, I32, I32, P, I64, P, I64, P, I64, P]),
+    "mdx_linear_plan": (I32, [I32, I64, I32, I32, I32, I32, I32]),
     "mdx_linear_backward_workspace_bytes": (I64, [I64, I32, I32, I32, I32, I32, I32, I32, I32]),
     "mdx_linear_backward": (I32, [P, I64, P, I64, P, I64, P, I64, I64, I32, I32, I32, I32, P, I64, P, I64, P, P, I64,
                                   P, I64, P]),

@@ -1215,7 +1215,7 @@ __device__ __forceinline__ void bias_join(const ActArgs &g, float *db, int block
 __global__ __launch_bounds__(256) void k_bias_join(ActArgs g, float *db) { bias_join(g, db, blockIdx.x); }
 
 // ---- kernels ----------------------------------------------------------------
-enum Kind { LARGE, DMA128, DMA64, REG128, REG64 };
+enum Kind { LARGE, DMA128, DMA64, REG128, REG64 };  // MDX_LINEAR_* in mdx.h
 constexpr int tile_side(int kind) { return kind == LARGE ? BIG : kind == DMA128 || kind == REG128 ? 128 : 64; }
 constexpr int tile_threads(int kind) { return kind == LARGE ? 512 : 256; }
 template <typename T> constexpr int tile_lds(int kind) {
@@ -1782,6 +1782,17 @@ extern "C" int mdx_linear(const void *x, int64_t ldx, const void *w, int64_t ldw
     g.act = act;
     g.part = reinterpret_cast<float *>(workspace);
     return run_forward("mdx_linear", p, g, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int mdx_linear_plan(int E, int64_t T, int N, int K, int dtype, int aligned, int backward) {
+    const Shape p{T, E, N, K, dtype, 0};
+    if (int rc = check_shape("mdx_linear_plan", p)) return rc;
+    if (backward) {
+        const Choice c = plan_backward(p, true, true, false, false, aligned).products;
+        return c.kind + 16 * c.splits;
+    }
+    const Plan q = plan_forward(p, aligned, PART_MAX);
+    return (q.few ? MDX_LINEAR_FEW : q.c.kind) + 16 * q.splits();
 }
 
 extern "C" int64_t mdx_linear_backward_workspace_bytes(int64_t M, int N, int K, int act, int dtype, int need_x,

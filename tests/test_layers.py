@@ -286,3 +286,26 @@ def test_negative_views(L):
         assert L._laid(t)[1] == shape[1] and L._rows(t, copy=False) is None
     t = torch._neg_view(torch.ones(3, 4))  # contiguous
     assert torch.equal(L._laid(t)[0], -torch.ones(3, 4)) and not L._laid(t)[0].is_neg() and not L._dense(t).is_neg()
+
+
+def test_plan(mdx):
+    """The kernel of a call: known to the caller, never one whose launch has 2^32 threads, and with slices that the
+    workspace has room for."""
+    from moseq2_detectron_extract_amd._lib import call
+    side, threads = (256, 128, 64, 128, 64), (512, 256, 256, 256, 256)
+    for M, N, K in ((1, 1, 1), (33, 8, 16), (1000, 1024, 12544), (2048, 2048, 2048), (6 * 10 ** 8, 8, 16),
+                    (12 * 10 ** 8, 8, 16), (2 ** 31 - 65537, 64, 1), (1, 54 * 10 ** 7, 8), (32, 2 ** 31 - 65537, 1)):
+        for dtype in (0, 1, 3):
+            room = call("mdx_linear_workspace_bytes", M, N, K, dtype)
+            for aligned in (0, 1):
+                kernel, slices = (lambda p: (p % 16, p // 16))(call("mdx_linear_plan", 0, M, N, K, dtype, aligned, 0))
+                assert kernel in ((5, 0, 1, 2) if aligned else (5, 3, 4)) and (kernel or dtype)
+                assert slices == 1 or slices * M * N * 4 <= room
+                if kernel < 5:
+                    tiles = -(-M // side[kernel]) * -(-N // side[kernel]) * slices
+                    assert tiles * threads[kernel] < 2 ** 32, (M, N, K, dtype, aligned, kernel)
+    assert call("mdx_linear_plan", 0, 4, 1024, 1024, 3, 1, 0) % 16 == 5
+    assert call("mdx_linear_plan", 0, 8192, 4096, 1024, 3, 1, 1) % 16 == 0
+    assert call("mdx_linear_plan", 8, 64, 4096, 1024, 0, 1, 0) % 16 == 5
+    for args in ((0, 4, 0, 8, 3, 1, 0), (4097, 4, 8, 8, 3, 1, 0), (0, 4, 8, 8, 2, 1, 0), (0, -1, 8, 8, 3, 1, 0)):
+        assert _refused("mdx_linear_plan", *args)[0] == -1

@@ -908,3 +908,125 @@ def test_c_entry_splits_whole_or_not(L, mdx, dt, M, N, K):
             assert torch.equal(out, once if untouched else whole), n
     need = min(n for n, u in seen.items() if not u)  # one size on which it turns, that of whole slices
     assert need % (4 * M * N) == 0 and all(u == (n < need) for n, u in seen.items()), seen
+
+
+# Every kernel of csrc/linear.hip by name (mdx_linear_plan), whole reductions and split ones, each at a shape that
+# is given to it: (kernel, split, dtypes, M, N, K).  Odd sizes end inside a tile, a piece and a step.
+KERNELS = ["256", "128", "64", "128 any", "64 any", "few"]
+HALF = [F16, BF16]
+
+
+def plan(E, T, N, K, dt, backward):
+    from moseq2_detectron_extract_amd._lib import call
+    n = 16 // dt.itemsize
+    aligned = K % n == 0 and (not backward or N % n == 0)
+    p = call("mdx_linear_plan", E, T, N, K, {F32: 0, F16: 1, BF16: 3}[dt], aligned, backward)
+    return KERNELS[p % 16], p // 16 > 1
+
+
+def each_type(cases):
+    return [pytest.param(k, split, dt, *shape, id=f"{k}{'-split' if split else ''}-{str(dt)[6:]}-{'x'.join(map(str, shape[:4]))}")
+            for k, split, dts, *shape in cases for dt in dts]
+
+
+@pytest.mark.parametrize("kernel,split,dt,M,N,K", each_type([
+    ("256", False, HALF, 2048, 4104, 520), ("256", True, HALF, 1000, 2056, 4104),
+    ("128", False, DTYPES, 1000, 2056, 264), ("128", True, [F32], 1000, 1000, 4100),
+    ("64", False, DTYPES, 300, 264, 264), ("64", True, DTYPES, 300, 264, 2056),
+    ("128 any", False, DTYPES, 4000, 1027, 263), ("128 any", True, HALF, 1001, 1003, 4097),
+    ("128 any", True, [F32], 515, 1990, 2047),
+    ("64 any", False, DTYPES, 301, 2049, 515), ("64 any", True, DTYPES, 301, 257, 1027),
+    ("few", False, DTYPES, 20, 4100, 264), ("few", True, DTYPES, 20, 40, 8200)]))
+def test_each_kernel_forward(L, kernel, split, dt, M, N, K):
+    assert plan(0, M, N, K, dt, 0) == (kernel, split)
+    g = gen(M + N + K)
+    x, w, b = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, N)
+    r = normal(g, M, N, dtype=dt)
+    for act in ("none", ACTS[1 + (M + K) % 4]):
+        y, pre = L.linear(x.cuda(), w.cuda(), b.cuda(), r.cuda(), act, return_pre=True)
+        check_forward(y, pre, x, w, b, r, act, dt)
+
+
+@pytest.mark.parametrize("kernel,split,dt,M,N,K", each_type([
+    ("256", False, HALF, 2048, 2056, 2088), ("256", True, HALF, 1000, 264, 8200), ("256", True, HALF, 4096, 1024, 1024),
+    ("128", False, DTYPES, 300, 264, 4104), ("128", True, [F32], 1000, 264, 4104), ("128", True, HALF, 4000, 1000, 520),
+    ("64", False, DTYPES, 300, 264, 520), ("64", True, [F32], 1000, 264, 520), ("64", True, HALF, 2100, 264, 520),
+    ("128 any", False, DTYPES, 300, 261, 8195),
+    ("128 any", True, DTYPES, 1001, 261, 4097), ("64 any", False, DTYPES, 301, 261, 517),
+    ("64 any", True, HALF, 1001, 261, 517), ("64 any", True, [F32], 515, 261, 517)]))
+def test_each_kernel_backward(L, kernel, split, dt, M, N, K):
+    """Without an activation dz is the gradient itself, so that each product's bound is that of its sum."""
+    assert plan(0, M, N, K, dt, 1) == (kernel, split)
+    g = gen(M + N + K)
+    x, w = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5)
+    dy, z = normal(g, M, N, dtype=dt), normal(g, M, N, dtype=dt)
+    for act in ("none", ACTS[1 + (M + K) % 4]):
+        got = L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), z.cuda(), act, need_bias=True, need_residual=True)
+        check_backward(got, dy, x, w, z, act, dt)
+
+
+def uneven(E, T):
+    """T rows in E groups: the second empty, the third of one row, the rest growing, the first with most."""
+    c = [0, 0, 1] + [k + 1 for k in range(E - 3)] if E > 3 else [0, 0, 1][:E]
+    if E > 3:
+        c = c[:3] + [v * (T // 3) // sum(c[3:]) for v in c[3:]]
+    c[0] = T - sum(c) - 5
+    return c
+
+
+@pytest.mark.parametrize("kernel,split,dt,E,T,N,K", each_type([
+    ("256", False, HALF, 3, 4099, 2056, 264), ("128", False, DTYPES, 2, 8195, 264, 264), ("64", False, DTYPES, 4, 1003, 264, 264),
+    ("128 any", False, HALF, 3, 4099, 2051, 519),
+    ("128 any", False, [F32], 3, 1003, 4001, 263), ("64 any", False, DTYPES, 4, 1003, 261, 263),
+    ("few", False, DTYPES, 4, 7, 72, 8200)]))
+def test_each_kernel_grouped_forward(L, kernel, split, dt, E, T, N, K):
+    assert plan(E, T, N, K, dt, 0) == (kernel, split)
+    x, w, b, r, _ = grouped_inputs(T, E, N, K, dt, T + E + N)
+    counts = uneven(E, T) if T > 100 else [2, 0, 1, 2]
+    sp, end = spans(counts, T)
+    x[end:] = float("nan")
+    cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    for act in ("none", ACTS[1 + (T + K) % 4]):
+        y = L.grouped_linear(x.cuda(), cd, w.cuda(), b.cuda(), r.cuda(), act).cpu()
+        for e, (s, t) in enumerate(sp):
+            check_forward(y[s:t], None, x[s:t], w[e], b[e], r[s:t], act, dt)
+        assert (y[end:] == 0).all()
+
+
+@pytest.mark.parametrize("kernel,split,dt,E,T,N,K", each_type([
+    ("256", False, HALF, 8, 2051, 1032, 1032), ("256", True, HALF, 8, 8192, 264, 520), ("256", True, HALF, 2, 16384, 1024, 512),
+    ("128", False, DTYPES, 5, 1003, 264, 1032), ("128", True, [F32], 8, 8192, 256, 512), ("128", True, HALF, 2, 8195, 264, 520),
+    ("64", False, DTYPES, 3, 1003, 264, 264), ("64", True, [F32], 2, 2051, 264, 264), ("64", True, HALF, 2, 4099, 264, 264),
+    ("128 any", False, HALF, 8, 1003, 515, 521), ("128 any", False, [F32], 5, 1003, 1001, 521),
+    ("128 any", True, [F32], 3, 4003, 515, 1031), ("128 any", True, HALF, 2, 4099, 261, 521),
+    ("64 any", False, DTYPES, 5, 1003, 261, 263), ("64 any", True, [F32], 2, 2051, 261, 263),
+    ("64 any", True, HALF, 2, 2051, 261, 263)]))
+def test_each_kernel_grouped_backward(L, kernel, split, dt, E, T, N, K):
+    """dW's slices of a group, of an empty one and of one row too, and each gradient alone."""
+    assert plan(E, T, N, K, dt, 1) == (kernel, split)
+    x, w, _, z, dy = grouped_inputs(T, E, N, K, dt, T + E + N + 1)
+    counts = uneven(E, T)
+    sp, end = spans(counts, T)
+    for t in (x, z, dy):
+        t[end:] = float("nan")
+    cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    a = (dy.cuda(), x.cuda(), cd, w.cuda(), z.cuda())
+    for act in ("none", ACTS[1 + (T + K) % 4]):
+        got = L.grouped_linear_backward(*a, act, need_bias=True, need_residual=True)
+        here = type(got)(*(t.cpu() for t in got))
+        for e, (s, t) in enumerate(sp):
+            check_backward(L_grads(here, e, s, t), dy[s:t], x[s:t], w[e], z[s:t], act, dt)
+        assert (here.x[end:] == 0).all() and (here.residual[end:] == 0).all()
+        for k, name in enumerate(("x", "weight", "bias", "residual")):
+            one = L.grouped_linear_backward(*a, act, **{f"need_{n}": n == name for n in ("x", "weight", "bias", "residual")})
+            assert torch.equal(one[k], got[k]) and all(o is None for i, o in enumerate(one) if i != k)
+
+
+@pytest.mark.parametrize("dt", HALF)
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_shapes_backward(L, dt, shape):
+    """The shapes of partial K-tiles backward, with the bound of the products' sums alone."""
+    M, N, K = shape
+    g = gen(M + N + K + 1)
+    x, w, dy = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, M, N, dtype=dt)
+    check_backward(L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), need_bias=True), dy, x, w, None, "none", dt, residual=False)
