@@ -643,7 +643,7 @@ int mdx_grouped_linear_backward(const void *grad, int64_t ldg, const void *x, in
 /* Layer norm of rows of D: out = (x - mean) rstd gamma + beta, biased
  * variance, rstd = 1 / sqrt(var + eps).  gamma / beta [D] or NULL (1 / 0).
  * mean / rstd [rows] or NULL: written for the backward pass.  out may be x's
- * own buffer (same ldo). */
+ * own buffer (same ldo).  Rows of more than 16384 elements: at most 2^22 - 1. */
 int mdx_layer_norm(const void *x, int64_t ldx, const float *gamma, const float *beta, int64_t rows, int D, float eps,
                    int dtype, void *out, int64_t ldo, float *mean, float *rstd, mdx_stream_t stream);
 /* dx (or NULL), dgamma = sum over rows of grad (x - mean) rstd (or NULL),

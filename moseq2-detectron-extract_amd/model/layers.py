@@ -218,6 +218,12 @@ def _limits(rows: int, *widths: int) -> None:
         raise ValueError(f"at most {_MOST} rows and columns")
 
 
+def _norm_limits(rows: int, D: int) -> None:
+    _limits(0, D)
+    if D > 16384 and rows >= 2 ** 22:
+        raise ValueError(f"at most {2 ** 22 - 1} rows of more than 16384 elements")
+
+
 def _check_counts(counts, E: int, like: torch.Tensor) -> None:
     _check("counts", counts, like, torch.int32, (E,))
     if not counts.is_contiguous():
@@ -405,7 +411,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, *, return_stats: bo
     _check("out", out, x, shape=x.shape)
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    _limits(0, D)
+    _norm_limits(x.numel() // D, D)
     _check_run(x, weight, bias, out)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -441,7 +447,7 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, *, need_x: bool = True
     _check("mean", mean, x, torch.float32, x.shape[:-1])
     _check("rstd", rstd, x, torch.float32, x.shape[:-1])
     _check("weight", weight, x, torch.float32, (D,))
-    _limits(0, D)
+    _norm_limits(x.numel() // D, D)
     _check_run(x, grad, mean, rstd, weight)
     if _elsewhere(x):
         with torch.cuda.device(x.device):

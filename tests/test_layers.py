@@ -309,3 +309,16 @@ def test_plan(mdx):
     assert call("mdx_linear_plan", 8, 64, 4096, 1024, 0, 1, 0) % 16 == 5
     for args in ((0, 4, 0, 8, 3, 1, 0), (4097, 4, 8, 8, 3, 1, 0), (0, 4, 8, 8, 2, 1, 0), (0, -1, 8, 8, 3, 1, 0)):
         assert _refused("mdx_linear_plan", *args)[0] == -1
+
+
+def test_layer_norm_refuses_many_wide_rows(L):
+    """A workgroup for each row of more than 16384 elements: 2^22 of them are refused (an expanded tensor: no memory)."""
+    x, s = z(1, 1, dtype=F32).expand(1 << 22, 16385), z(1, dtype=F32).expand(1 << 22)
+    with pytest.raises(ValueError, match="rows of more than 16384"):
+        L.layer_norm(x)
+    with pytest.raises(ValueError, match="rows of more than 16384"):
+        L.layer_norm_backward(x, x, s, s)
+    with pytest.raises(ValueError, match="GPU"):
+        L.layer_norm(x[1:])
+    with pytest.raises(ValueError, match="GPU"):
+        L.layer_norm(z(1, 1, dtype=F32).expand(1 << 22, 16384))

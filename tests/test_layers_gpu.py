@@ -1030,3 +1030,29 @@ def test_large_shapes_backward(L, dt, shape):
     g = gen(M + N + K + 1)
     x, w, dy = normal(g, M, K, dtype=dt), normal(g, N, K, dtype=dt, scale=K ** -0.5), normal(g, M, N, dtype=dt)
     check_backward(L.linear_backward(dy.cuda(), x.cuda(), w.cuda(), need_bias=True), dy, x, w, None, "none", dt, residual=False)
+
+
+def test_layer_norm_backward_very_wide(L):
+    """More columns than a launch has threads for in the sums' join (2^26) and, of rows, in both passes (2^30)."""
+    def check(R, D, dx):
+        g = torch.Generator(device="cuda").manual_seed(D)
+        x, dy = (torch.empty(R, D, dtype=BF16, device="cuda").normal_(generator=g) for _ in range(2))
+        mean, rstd = torch.full((R,), 0.125, device="cuda"), torch.full((R,), 0.5, device="cuda")
+        got = L.layer_norm_backward(dy, x, mean, rstd, need_x=dx)
+        for c in range(0, D, 1 << 26):  # columns c ..
+            part = slice(c, min(D, c + (1 << 26)))
+            h, d = (x[:, part].double() - 0.125) * 0.5, dy[:, part].double()
+            for a, want, size in ((got.weight, (d * h).sum(0), (d * h).abs().sum(0)), (got.bias, d.sum(0), d.abs().sum(0))):
+                assert ((a[part].double() - want).abs() <= (R + 8) * V * size).all()
+        return got.x, x, dy
+    D = (1 << 26) + 25
+    dx, x, dy = check(2, D, True)
+    X, DY = x.double(), dy.double()
+    h = (X - 0.125) * 0.5
+    s1, s2 = DY.mean(1, keepdim=True), (DY * h).mean(1, keepdim=True)
+    want = 0.5 * (DY - s1 - h * s2)
+    c = chain(D) * V  # of sums of random signs: some thousandth of the terms' size over its root
+    e = 0.5 * (c * DY.abs().mean(1, keepdim=True) + h.abs() * (c * (DY * h).abs().mean(1, keepdim=True)) + 8 * V * (DY.abs() + h.abs()))
+    assert ((dx.double() - want).abs() <= e + unit(BF16) * (want.abs() + e)).all()
+    del dx, x, dy, X, DY, h, want, e
+    check(1, (1 << 30) + 77, False)
