@@ -12,4 +12,8 @@ def __getattr__(name):
     if name in ("Predictor", "outputs_to_instances"):
         from . import predict
         return getattr(predict, name)
+    if name in ("linear", "linear_backward", "grouped_linear", "grouped_linear_backward", "layer_norm",
+                "layer_norm_backward"):
+        import importlib
+        return getattr(importlib.import_module(".layers", __name__), name)
     raise AttributeError(name)

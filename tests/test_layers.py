@@ -322,3 +322,13 @@ def test_layer_norm_refuses_many_wide_rows(L):
         L.layer_norm(x[1:])
     with pytest.raises(ValueError, match="GPU"):
         L.layer_norm(z(1, 1, dtype=F32).expand(1 << 22, 16384))
+
+
+def test_layers_are_exported(L):
+    """The layers are reached from the model package, as the runtime and the predictor are."""
+    from moseq2_detectron_extract_amd import model
+    for name in ("linear", "linear_backward", "grouped_linear", "grouped_linear_backward", "layer_norm", "layer_norm_backward"):
+        assert getattr(model, name) is getattr(L, name)
+    from moseq2_detectron_extract_amd.model import layer_norm, linear  # noqa: F401
+    with pytest.raises(AttributeError):
+        model.other
