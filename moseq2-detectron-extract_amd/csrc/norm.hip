@@ -9,49 +9,19 @@
 // there in float32 (the variance in a second pass over the registers, around
 // the mean), and the result is written once.  Rows wider than the registers
 // of a workgroup hold are read again instead (k_norm_wide*).
-#include "common.h"
+#include "pieces.h"
 
 #include <algorithm>
 
 namespace mdx {
 namespace norm {
 
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Un16 { u4 v; };  // rows start anywhere
-template <typename T> constexpr int VEC = 16 / (int)sizeof(T);
-
 template <typename T> struct Piece {
     union { u4 u; T e[VEC<T>]; };
 };
-// 16 bytes shifted down by s bits, 0 <= s < 128
-__device__ __forceinline__ u4 shift_down(u4 v, int s) {
-    union { u4 u; unsigned long long d[2]; } r;
-    r.u = v;
-    if (s >= 64) {
-        r.d[0] = r.d[1];
-        r.d[1] = 0;
-        s -= 64;
-    }
-    if (s) {
-        r.d[0] = r.d[0] >> s | r.d[1] << (64 - s);
-        r.d[1] >>= s;
-    }
-    return r.u;
-}
-// the piece at a row's element c, of which the first n elements exist (n <= 0:
-// none); the rest is 0.  The last piece of a row is read as the 16 bytes that
-// end with it, shifted down.
 template <typename T> __device__ __forceinline__ Piece<T> load(const T *p, int c, int n) {
     Piece<T> r;
-    r.u = u4{0, 0, 0, 0};
-    if (n >= VEC<T>)
-        r.u = reinterpret_cast<const Un16<T> *>(p)->v;
-    else if (n > 0 && c + n >= VEC<T>)
-        r.u = shift_down(reinterpret_cast<const Un16<T> *>(p - (VEC<T> - n))->v, (VEC<T> - n) * 8 * (int)sizeof(T));
-    else
-#pragma unroll
-        for (int q = 0; q < VEC<T>; ++q)
-            if (q < n) r.e[q] = p[q];
+    r.u = load_piece(p, c, n);
     return r;
 }
 template <typename T> __device__ __forceinline__ void store(T *p, const Piece<T> &v, int n) {
