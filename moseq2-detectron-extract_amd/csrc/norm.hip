@@ -367,9 +367,11 @@ template <typename T> __global__ __launch_bounds__(1024) void k_norm_wide_backwa
         store(o + c, z, (int)(a.D - c));
     }
 }
-// dg and db of any width: a workgroup takes 64 columns of one slice of the rows
-// at a time, and goes on where a launch has no threads for all columns
-template <typename T> __device__ __forceinline__ void wide_sums(const Args &a, long long c, float (&sh)[2][256]) {
+// dg and db of any width, from column `first` on: a workgroup takes 64 columns
+// of one slice of the rows
+template <typename T> __global__ __launch_bounds__(256) void k_norm_wide_sums(Args a, int first) {
+    __shared__ float sh[2][256];
+    const long long c = first + (long long)blockIdx.x * 64 + (threadIdx.x & 63);
     const long long per = (a.rows + gridDim.y - 1) / gridDim.y, r1 = min(a.rows, (blockIdx.y + 1) * per);
     float dg = 0.f, db = 0.f;
     if (c < a.D)
@@ -378,7 +380,6 @@ template <typename T> __device__ __forceinline__ void wide_sums(const Args &a, l
             dg += e * (((float)reinterpret_cast<const T *>(a.x)[r * a.ldx + c] - a.mean[r]) * a.rstd[r]);
             db += e;
         }
-    __syncthreads();  // the sums before these have been read
     sh[0][threadIdx.x] = dg;
     sh[1][threadIdx.x] = db;
     __syncthreads();
@@ -388,50 +389,42 @@ template <typename T> __device__ __forceinline__ void wide_sums(const Args &a, l
         if (c < a.D) a.part[((long long)blockIdx.y * 2 + k) * a.D + c] = v;
     }
 }
-template <typename T> __global__ __launch_bounds__(256) void k_norm_wide_sums(Args a) {
-    __shared__ float sh[2][256];
-    for (long long c = (long long)blockIdx.x * 64; c < a.D; c += (long long)gridDim.x * 64)
-        wide_sums<T>(a, c + (threadIdx.x & 63), sh);
-}
 // dg, db = the workgroups' shares, always added in the same order.  16 columns
 // to a workgroup and 64 threads to each: a few loads in flight per thread and
 // no chain of waits (64 columns and 16 threads to each took 11 us for 512
-// shares of 1024 columns).
-__global__ __launch_bounds__(1024) void k_norm_join(const float *part, int n, int D, float *dg, float *db) {
+// shares of 1024 columns).  From column `first` on.
+__global__ __launch_bounds__(1024) void k_norm_join(const float *part, int n, int D, float *dg, float *db, int first) {
     __shared__ float sh[16][16];
     const int l = threadIdx.x & 15, w = threadIdx.x >> 4, k = blockIdx.y;
+    const long long c = first + (long long)blockIdx.x * 16 + l;
     float *o = k ? db : dg;
     if (!o) return;
-    for (long long c0 = (long long)blockIdx.x * 16; c0 < D; c0 += (long long)gridDim.x * 16) {
-        const long long c = c0 + l;
-        float v = 0.f;
-        if (c < D)
-            for (int s = w; s < n; s += 8 * 64) {
-                float t[8];
+    float v = 0.f;
+    if (c < D)
+        for (int s = w; s < n; s += 8 * 64) {
+            float t[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    t[q] = s + 64 * q < n ? part[((long long)(s + 64 * q) * 2 + k) * D + c] : 0.f;
+            for (int q = 0; q < 8; ++q) t[q] = s + 64 * q < n ? part[((long long)(s + 64 * q) * 2 + k) * D + c] : 0.f;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v += t[q];
-            }
-        v += __shfl_xor(v, 16);
-        v += __shfl_xor(v, 32);
-        __syncthreads();  // the sums before these have been read
-        if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][l] = v;
-        __syncthreads();
-        if (threadIdx.x < 16 && c < D) {
-            v = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v += sh[i][l];
-            o[c] = v;
+            for (int q = 0; q < 8; ++q) v += t[q];
         }
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    if ((threadIdx.x & 63) < 16) sh[threadIdx.x >> 6][l] = v;
+    __syncthreads();
+    if (threadIdx.x < 16 && c < D) {
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += sh[i][l];
+        o[c] = v;
     }
 }
 
 // ---- host ---------------------------------------------------------------
-// workgroups of a kernel that goes on by itself: a launch has fewer than 2^32
-// threads in each direction
-static unsigned blocks_of(long long n, int threads) { return (unsigned)std::min<long long>(n, (1u << 31) / threads); }
+// Columns of one launch where `per` threads work on each: a launch has fewer
+// than 2^32 threads in each direction, so very wide rows (above 2^25 columns in
+// k_norm_join, 2^29 in k_norm_wide_sums) take several.
+static long long columns_of(int per) { return (1ll << 31) / per; }
 // The layout of rows of D elements: the first of these that holds their pieces
 // of 16 bytes, 0 for wider ones.  A thread's pieces stay in registers, forward
 // next to gamma and beta, backward next to gamma and the sums of dg and db, so
@@ -504,7 +497,9 @@ template <typename T> static void run_backward(const Args &a, int lay, int group
     }
     // the sums first: dx may be written over dy
     if (a.part)
-        hipLaunchKernelGGL(k_norm_wide_sums<T>, dim3(blocks_of(ceil_div(a.D, 64), 256), groups), dim3(256), 0, s, a);
+        for (long long c = 0, n = columns_of(4); c < a.D; c += n)
+            hipLaunchKernelGGL(k_norm_wide_sums<T>, dim3((unsigned)ceil_div(std::min(n, a.D - c), 64), groups), dim3(256), 0,
+                               s, a, (int)c);
     if (a.out && a.rows)
         hipLaunchKernelGGL(k_norm_wide_backward<T>, dim3((unsigned)a.rows), dim3(1024), 0, s, a);
 }
@@ -517,8 +512,9 @@ template <typename T> static int run(const char *fn, const Args &a, int dtype, b
         run_forward<T>(a, lay, s);
     MDX_CHECK_LAUNCH(fn);
     if (back && a.part) {
-        hipLaunchKernelGGL(k_norm_join, dim3(blocks_of(ceil_div(a.D, 16), 1024), 2), dim3(1024), 0, s, a.part, groups, a.D,
-                           dg, db);
+        for (long long c = 0, n = columns_of(64); c < a.D; c += n)
+            hipLaunchKernelGGL(k_norm_join, dim3((unsigned)ceil_div(std::min(n, a.D - c), 16), 2), dim3(1024), 0, s, a.part,
+                               groups, a.D, dg, db, (int)c);
         MDX_CHECK_LAUNCH(fn);
     }
     return MDX_OK;

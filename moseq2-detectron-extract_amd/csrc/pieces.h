@@ -30,12 +30,12 @@ __device__ __forceinline__ u4 shift_down(u4 v, int s) {
 // 16 bytes of a row from its element c on, of which the first n exist (n <= 0:
 // none); the rest is zero.  The last piece of a row is read as the 16 bytes
 // that end with it, shifted down.
-template <typename T> __device__ __forceinline__ u4 load_piece(const T *p, long long c, long long n) {
+template <typename T> __device__ __forceinline__ u4 load_piece(const T *p, int c, int n) {
     constexpr int N = VEC<T>;
     if (n >= N) return reinterpret_cast<const Un16<T> *>(p)->v;
     if (n <= 0) return u4{0, 0, 0, 0};
     if (c + n >= N)
-        return shift_down(reinterpret_cast<const Un16<T> *>(p - (N - n))->v, (int)(N - n) * 8 * (int)sizeof(T));
+        return shift_down(reinterpret_cast<const Un16<T> *>(p - (N - n))->v, (N - n) * 8 * (int)sizeof(T));
     union { u4 u; T e[N]; } r;
     r.u = u4{0, 0, 0, 0};
 #pragma unroll
