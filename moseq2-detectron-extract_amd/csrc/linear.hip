@@ -16,7 +16,7 @@
 // 8192 x 4096 x 1024 GELU are off by 0.0023 of their size on the whole, where rounded
 // outputs alone give 0.0017; fp16 999 x 517 x 1001 SiLU 2.9e-4 and 2.1e-4).  A dz in
 // two parts would keep the rest for twice the products' time (8192 x 4096 x 1024:
-// 111 us); between separate layers of the type it is rounded just so.  In fp16
+// 113 us); between separate layers of the type it is rounded just so.  In fp16
 // it shares the type's range: beyond 65504 infinite, below 2^-25 zero.
 #include "pieces.h"
 
@@ -837,7 +837,8 @@ __device__ __forceinline__ void small_product(const Args &g, char *lds, int id) 
 // meet in LDS.  Rows and columns beyond the end are clamped: their products are
 // not stored.  Bound by the weight's way from memory, in small layers by the
 // chain of launch, load and join: bf16 1 x 4096 x 4096 8.1 us (4.2 TB/s), 16 x 1024
-// x 12544 in slices 12.1 (2.1 TB/s), 4 x 1024 x 1024 3.9.
+// x 12544 in slices 12.1 (2.1 TB/s), 4 x 1024 x 1024 3.9 (from call to call in a
+// graph; a trace has 4.5 for that kernel alone).
 template <typename T, int MODE, int MT, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_product_few(Args g) {
     constexpr int N = VEC<T>, KC = 8 * N, U = 4, ROWS = 16 * MT, COLS = 16 * NT;
@@ -1201,7 +1202,7 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_forward(Args g) {
 }
 // dW's tiles and dx's in one launch: they need nothing of each other, and
 // either alone often leaves part of the CUs without a tile (8192 x 4096 x 1024
-// bf16: 111 us for both, 2 x 69 GFLOP at 1.24 PFLOP/s).  Of dW's nw tiles
+// bf16: 113 us for both, 2 x 69 GFLOP at 1.22 PFLOP/s).  Of dW's nw tiles
 // the `first` ones come before dx's, whose reduction is x.R: those that reduce
 // more (grouped: of the groups with more rows).  The bias's blocks come last.
 template <typename T, bool GROUPED, int KIND>
@@ -1226,7 +1227,7 @@ __global__ __launch_bounds__(tile_threads(KIND), 2) void k_backward(Args w, int 
 
 // The slices' partial sums, added in their order (no atomics: the same result
 // on every call), and the epilogue; one thread per 16 bytes of output.  Bound by
-// HBM: four slices of 4096 x 1024 8.8 us (8.6 TB/s from the L2s and beyond).
+// HBM: two slices of 4096 x 1024 to bf16 8.7 us for their 42 MB (4.8 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void k_product_join(Args g) {
     constexpr int N = VEC<T>;
