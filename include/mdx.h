@@ -577,8 +577,9 @@ enum {
     MDX_ACT_SILU = 4        /* z / (1 + exp(-z)) */
 };
 /* Before its rounding an activation is within 16 * 2^-24 (float32) or 4e-5
- * (16-bit types) of its value, far tails included; its slope within as much of
- * the gate and of z times the gate's slope. */
+ * (16-bit types) of its value, far tails included as long as the gate (what z is
+ * multiplied with) is a normal float32 number; its slope within as much of the
+ * gate and of z times the gate's slope. */
 
 /* z = x w^T + bias + residual; out = act(z); pre (or NULL) = z.
  * x (M,K), w (N,K), bias [N] or NULL, residual (M,N) or NULL, out / pre (M,N).
